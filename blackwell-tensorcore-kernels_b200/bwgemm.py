@@ -12,6 +12,7 @@ Reference interface mirrored (paths within waynehacking8/blackwell-tensorcore-ke
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import os
 import re
@@ -27,7 +28,7 @@ OUT_F32, OUT_BF16 = 0, 1
 SCALE_NONE, SCALE_FIXED8, SCALE_AMAX = 0, 1, 2
 FP4_PACKED, FP4_BYTE_SHL2 = 0, 1
 MX_UNIT_FIXED8, MX_BLOCK32 = 0, 1
-DTYPE_F16, DTYPE_FP8, DTYPE_FP4, DTYPE_MXFP4 = 0, 1, 2, 3
+DTYPE_F16, DTYPE_FP8, DTYPE_FP4, DTYPE_MXFP4, DTYPE_BF16, DTYPE_F32 = 0, 1, 2, 3, 4, 5
 
 
 class Shard(ctypes.Structure):
@@ -69,6 +70,7 @@ def lib():
         raise RuntimeError(f"{LIB_PATH} is missing: run __graft_entry__.build() (make -C {_HERE})")
     L = ctypes.CDLL(LIB_PATH)
     P, I, LL = ctypes.c_void_p, ctypes.c_int, ctypes.c_longlong
+    F, SZ = ctypes.c_float, ctypes.c_size_t
     sig = {
         "bw_init": [I],
         "bw_shutdown": [],
@@ -89,6 +91,9 @@ def lib():
         "bw_quantize_fp8_noalloc": [P, P, P, I, I, I, I, P],
         "bw_quantize_fp4": [P, P, P, I, I, I, I, I, P],
         "bw_quantize_mxfp4": [P, P, P, I, I, I, I, P],
+        "bw_rmsnorm": [P, LL, P, LL, P, I, I, F, P, LL, P, LL, P, I, I, P],
+        "bw_rmsnorm_fp8": [P, LL, P, LL, P, I, I, F, P, LL, P, P, LL, P, I, I, P],
+        "bw_rmsnorm_backward": [P, LL, P, LL, P, I, I, P, P, LL, P, LL, P, P, SZ, I, I, P],
         "bw_unshard_columns": [P, P, I, I, I, P],
         "bw_unshard_columns_bf16": [P, P, I, I, I, P],
         "bw_gemm_sharded": [I, I, P, I, I, I, I, I],
@@ -109,6 +114,8 @@ def lib():
     L.bw_last_error_string.restype = ctypes.c_char_p
     L.bw_sf_bytes.argtypes = [I, I]
     L.bw_sf_bytes.restype = ctypes.c_size_t
+    L.bw_rmsnorm_backward_workspace.argtypes = [I, I]
+    L.bw_rmsnorm_backward_workspace.restype = ctypes.c_size_t
     L.bw_sf_offset.argtypes = [I, I, I]
     L.bw_sf_offset.restype = ctypes.c_size_t
     _lib = L
@@ -281,6 +288,146 @@ def quantize_mxfp4(src, transpose=False, mode=MX_BLOCK32, dst=None, sf=None, str
     _check(lib().bw_quantize_mxfp4(_ptr(src), _ptr(dst), _ptr(sf), rows, cols, int(transpose), mode,
                                    _stream(stream)))
     return dst, sf
+
+
+# ------------------------------------------------------------------ root-mean-square norm
+def _dtype_code(t, what: str, allowed: tuple[str, ...]) -> int:
+    import torch
+
+    codes = {torch.float32: ("float32", DTYPE_F32), torch.float16: ("float16", DTYPE_F16),
+             torch.bfloat16: ("bfloat16", DTYPE_BF16), torch.uint8: ("uint8", DTYPE_FP8)}
+    name, code = codes.get(t.dtype, (str(t.dtype), -1))
+    if name not in allowed:
+        raise TypeError(f"{what} must be {' or '.join(allowed)}, not {name}")
+    return code
+
+
+def _need(what: str, t, shape: tuple, dtype, device, pitched: bool = True) -> int:
+    """Checks an operand's shape, type, device and layout; returns the row pitch of a 2-D one."""
+    if t.dtype != dtype:
+        raise TypeError(f"{what} must be {dtype}, not {t.dtype}")
+    if tuple(t.shape) != shape:
+        raise ValueError(f"{what} has shape {tuple(t.shape)}, expected {shape}")
+    if t.device != device:
+        raise ValueError(f"{what} is on {t.device}, expected {device}")
+    if len(shape) == 2 and pitched:
+        if shape[1] > 1 and t.stride(1) != 1:
+            raise ValueError(f"{what} must have contiguous rows (strides {t.stride()})")
+        return t.stride(0) if shape[0] > 1 else shape[1]
+    if not t.is_contiguous():
+        raise ValueError(f"{what} must be contiguous")
+    return 0
+
+
+_NO_SCOPE = contextlib.nullcontext()
+
+
+def _scope(device, stream):
+    """Makes `device` (the operands') and `stream` current: what a call allocates belongs to the
+    stream that it runs on."""
+    import torch
+
+    if device.type != "cuda":
+        raise ValueError(f"operands must be on a CUDA device, not {device}")
+    if stream is None:
+        return _NO_SCOPE if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+    if isinstance(stream, int):
+        stream = torch.cuda.ExternalStream(stream, device=device)
+    if stream.device != device:
+        raise ValueError(f"stream is of {stream.device}, operands are on {device}")
+    return torch.cuda.stream(stream)
+
+
+def _norm_operands(x, weight, residual):
+    if x.dim() != 2 or weight.dim() != 1:
+        raise ValueError(f"rmsnorm takes x (rows x cols) and weight (cols), not {x.dim()}-D and {weight.dim()}-D")
+    code = _dtype_code(x, "x", ("float32", "float16", "bfloat16"))
+    shape, dev = tuple(x.shape), x.device
+    ldx = _need("x", x, shape, x.dtype, dev)
+    wcode = DTYPE_F32 if weight.dtype.itemsize == 4 else code
+    import torch
+
+    _need("weight", weight, (shape[1],), torch.float32 if wcode == DTYPE_F32 else x.dtype, dev)
+    ldr = _need("residual", residual, shape, x.dtype, dev) if residual is not None else 0
+    return code, wcode, shape, dev, ldx, ldr
+
+
+def _norm_outputs(x, shape, dev, residual, h, rstd):
+    import torch
+
+    if h is None:
+        h = torch.empty(shape, dtype=x.dtype, device=dev) if residual is not None else x
+    ldh = _need("h", h, shape, x.dtype, dev)
+    if rstd is None:
+        rstd = torch.empty(shape[0], dtype=torch.float32, device=dev)
+    _need("rstd", rstd, (shape[0],), torch.float32, dev)
+    return h, ldh, rstd, None if h is x else h
+
+
+def rmsnorm(x, weight, residual=None, eps: float = 1e-6, y=None, h=None, rstd=None, stream=None):
+    """y = norm(h) * weight with h = x + residual (x without one); returns (y, h, rstd).
+
+    x, residual, y, h: rows x cols of float32, float16 or bfloat16 with contiguous rows; weight of
+    the same type or float32. h (x itself where there is no residual) and rstd are what
+    rmsnorm_backward takes. y and h may be x's or the residual's own tensor."""
+    import torch
+
+    code, wcode, shape, dev, ldx, ldr = _norm_operands(x, weight, residual)
+    with _scope(dev, stream):
+        h, ldh, rstd, hout = _norm_outputs(x, shape, dev, residual, h, rstd)
+        if y is None:
+            y = torch.empty(shape, dtype=x.dtype, device=dev)
+        ldy = _need("y", y, shape, x.dtype, dev)
+        _check(lib().bw_rmsnorm(_ptr(x), ldx, _ptr(residual), ldr, _ptr(weight), code, wcode, eps, _ptr(y), ldy,
+                                _ptr(hout), ldh, _ptr(rstd), shape[0], shape[1], _stream(None)))
+    return y, h, rstd
+
+
+def rmsnorm_fp8(x, weight, residual=None, eps: float = 1e-6, q=None, row_scale=None, h=None, rstd=None, stream=None):
+    """rmsnorm with E4M3 output: q (uint8 codes) and row_scale (float32, one a row) with
+    y = q * row_scale, as gemm_grouped takes them; returns (q, row_scale, h, rstd)."""
+    import torch
+
+    code, wcode, shape, dev, ldx, ldr = _norm_operands(x, weight, residual)
+    with _scope(dev, stream):
+        h, ldh, rstd, hout = _norm_outputs(x, shape, dev, residual, h, rstd)
+        if q is None:
+            q = torch.empty(shape, dtype=torch.uint8, device=dev)
+        ldq = _need("q", q, shape, torch.uint8, dev)
+        if row_scale is None:
+            row_scale = torch.empty(shape[0], dtype=torch.float32, device=dev)
+        _need("row_scale", row_scale, (shape[0],), torch.float32, dev)
+        _check(lib().bw_rmsnorm_fp8(_ptr(x), ldx, _ptr(residual), ldr, _ptr(weight), code, wcode, eps, _ptr(q), ldq,
+                                    _ptr(row_scale), _ptr(hout), ldh, _ptr(rstd), shape[0], shape[1], _stream(None)))
+    return q, row_scale, h, rstd
+
+
+def rmsnorm_backward(dy, h, weight, rstd, dresidual=None, dx=None, dweight=None, workspace=None, stream=None):
+    """Gradient of rmsnorm from the h and rstd it returned: (dx, dweight). dx is the gradient of x
+    and of the residual alike, with dresidual (the gradient that reached h past the norm) added;
+    dweight is float32. dx may be dy's, h's or dresidual's own tensor. `workspace`: uint8 tensor of
+    bw_rmsnorm_backward_workspace(rows, cols) bytes; one of the call's own where None."""
+    import torch
+
+    code, wcode, shape, dev, ldh, _ = _norm_operands(h, weight, None)
+    lddy = _need("dy", dy, shape, h.dtype, dev)
+    _need("rstd", rstd, (shape[0],), torch.float32, dev)
+    lddr = _need("dresidual", dresidual, shape, h.dtype, dev) if dresidual is not None else 0
+    with _scope(dev, stream):
+        if dx is None:
+            dx = torch.empty(shape, dtype=h.dtype, device=dev)
+        lddx = _need("dx", dx, shape, h.dtype, dev)
+        if dweight is None:
+            dweight = torch.empty(shape[1], dtype=torch.float32, device=dev)
+        _need("dweight", dweight, (shape[1],), torch.float32, dev)
+        if workspace is None:
+            workspace = torch.empty(lib().bw_rmsnorm_backward_workspace(*shape), dtype=torch.uint8, device=dev)
+        elif workspace.dtype != torch.uint8 or workspace.device != dev or not workspace.is_contiguous():
+            raise ValueError("workspace must be a contiguous uint8 tensor on the operands' device")
+        _check(lib().bw_rmsnorm_backward(_ptr(dy), lddy, _ptr(h), ldh, _ptr(weight), code, wcode, _ptr(rstd),
+                                         _ptr(dresidual), lddr, _ptr(dx), lddx, _ptr(dweight), _ptr(workspace),
+                                         workspace.numel(), shape[0], shape[1], _stream(None)))
+    return dx, dweight
 
 
 def unshard_columns(C_shardmajor, M: int, N: int, world: int, out=None, stream=None):

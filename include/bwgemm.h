@@ -153,6 +153,37 @@ int bw_quantize_mxfp4(const float* src, uint8_t* dst, uint8_t* sf, int rows, int
 size_t bw_sf_bytes(int outer, int K);
 size_t bw_sf_offset(int row, int kblock, int K);
 
+/* ---------------- root-mean-square norm ---------------- */
+/* No counterpart in the reference. For each of `rows` rows of `cols` elements (1 or more):
+ *   h = x + residual, rounded to x's type (residual NULL: h = x)
+ *   rstd = (mean(h^2) + eps)^(-1/2),   y = h * weight * rstd
+ * bw_rmsnorm writes y in x's type; bw_rmsnorm_fp8 writes E4M3 codes and one scale a row, as
+ * bw_gemm_grouped takes them: row_scale = amax(|y|) / 448 (1 when the maximum is 0, not finite, or so
+ * small that 448 / amax overflows), q = cvt(y * (448 / amax)), satfinite.
+ * dtype: BW_DTYPE_F32, F16 or BF16 (x, residual, y, h); weight_dtype: the same or BW_DTYPE_F32.
+ * h and rstd may be NULL (not wanted). ld*: row pitches in elements, at least cols. Any alignment
+ * to whole elements; 16-byte aligned rows run faster. y and h may be x's or the residual's own
+ * buffer (same type, same pitch); other overlap is not allowed. Sums are FP32: a row whose squares
+ * sum to more than FP32 holds gets rstd = 0, one with a NaN gets NaN (codes 0x7f, scale 1). */
+int bw_rmsnorm(const void* x, long long ldx, const void* residual, long long ldr, const void* weight, int dtype,
+               int weight_dtype, float eps, void* y, long long ldy, void* h, long long ldh, float* rstd, int rows,
+               int cols, void* stream);
+int bw_rmsnorm_fp8(const void* x, long long ldx, const void* residual, long long ldr, const void* weight, int dtype,
+                   int weight_dtype, float eps, uint8_t* q, long long ldq, float* row_scale, void* h, long long ldh,
+                   float* rstd, int rows, int cols, void* stream);
+/* Gradient, from the h and rstd that the forward call kept: with n = h * rstd,
+ *   dx = rstd * (dy * weight - n * mean(dy * weight * n)) + dresidual   (x's type; also the residual's gradient)
+ *   dweight = sum over rows of dy * n                                   (FP32, overwritten; zeros for rows = 0)
+ * dresidual (NULL: none) is the gradient that reached h past the norm. dx may be dy's, h's or
+ * dresidual's own buffer (same pitch). workspace: device memory of at least
+ * bw_rmsnorm_backward_workspace(rows, cols) bytes, the caller's own for as long as the call runs on
+ * the stream (calls that may overlap need one each). Rows are summed in an order fixed by the sizes. */
+size_t bw_rmsnorm_backward_workspace(int rows, int cols);
+int bw_rmsnorm_backward(const void* dy, long long lddy, const void* h, long long ldh, const void* weight, int dtype,
+                        int weight_dtype, const float* rstd, const void* dresidual, long long lddr, void* dx,
+                        long long lddx, float* dweight, void* workspace, size_t workspace_bytes, int rows, int cols,
+                        void* stream);
+
 /* ---------------- N-sharded multi-GPU GEMM helpers ---------------- */
 /* Column sharding (one process per GPU) needs no new GEMM: rank r calls bw_gemm_* on its
  * shard B[:, r*N/world:(r+1)*N/world]. When a gathered C is requested, the host layer
@@ -213,7 +244,7 @@ int bw_ipc_close(void* peer_ptr);
  * synchronise. Replaces nothing in the reference (it runs on one GPU, src/main.cu:47-111).
  * Returns BW_ERR_INVALID for bad arguments before touching any device, BW_ERR_UNSUPPORTED when
  * a gather is requested and NCCL cannot be loaded. */
-enum { BW_DTYPE_F16 = 0, BW_DTYPE_FP8 = 1, BW_DTYPE_FP4 = 2, BW_DTYPE_MXFP4 = 3 };
+enum { BW_DTYPE_F16 = 0, BW_DTYPE_FP8 = 1, BW_DTYPE_FP4 = 2, BW_DTYPE_MXFP4 = 3, BW_DTYPE_BF16 = 4, BW_DTYPE_F32 = 5 };
 typedef struct {
   int device;
   const void* A;
