@@ -94,6 +94,8 @@ def lib():
         "bw_rmsnorm": [P, LL, P, LL, P, I, I, F, P, LL, P, LL, P, I, I, P],
         "bw_rmsnorm_fp8": [P, LL, P, LL, P, I, I, F, P, LL, P, P, LL, P, I, I, P],
         "bw_rmsnorm_backward": [P, LL, P, LL, P, I, I, P, P, LL, P, LL, P, P, SZ, I, I, P],
+        "bw_gemm_grouped": [I, P, LL, P, I, P, I, P, P, P, LL, I, I, I, I, P],
+        "bw_gemm_grouped_wgrad": [I, P, LL, P, LL, P, I, P, I, I, I, I, P],
         "bw_unshard_columns": [P, P, I, I, I, P],
         "bw_unshard_columns_bf16": [P, P, I, I, I, P],
         "bw_gemm_sharded": [I, I, P, I, I, I, I, I],
@@ -428,6 +430,80 @@ def rmsnorm_backward(dy, h, weight, rstd, dresidual=None, dx=None, dweight=None,
                                          _ptr(dresidual), lddr, _ptr(dx), lddx, _ptr(dweight), _ptr(workspace),
                                          workspace.numel(), shape[0], shape[1], _stream(None)))
     return dx, dweight
+
+
+# ------------------------------------------------------------------ products grouped by expert
+def _out_type(out_dtype: int):
+    import torch
+
+    if out_dtype not in (OUT_F32, OUT_BF16):
+        raise ValueError(f"out_dtype must be OUT_F32 or OUT_BF16, not {out_dtype}")
+    return torch.bfloat16 if out_dtype == OUT_BF16 else torch.float32
+
+
+def _groups(offsets, dev) -> int:
+    import torch
+
+    if offsets.dim() != 1 or offsets.shape[0] < 2:
+        raise ValueError(f"offsets must hold groups + 1 ints, not a tensor of shape {tuple(offsets.shape)}")
+    _need("offsets", offsets, tuple(offsets.shape), torch.int32, dev)
+    return offsets.shape[0] - 1
+
+
+def gemm_grouped(A, B, offsets, C=None, b_transposed: bool = False, row_scale=None, group_scale=None,
+                 out_dtype=OUT_BF16, stream=None):
+    """C[r] = (A[r] x B[g]) * row_scale[r] * group_scale[g] for offsets[g] <= r < offsets[g + 1].
+
+    A: rows x K float16, bfloat16 or uint8 (E4M3 codes); B: groups x K x N, or groups x N x K with
+    b_transposed (E4M3: only that). offsets: groups + 1 int32 on the device. The product with the
+    other layout of B is the input gradient. Rows outside offsets[0]..offsets[groups] are left as
+    they were (a C allocated here holds arbitrary values there)."""
+    import torch
+
+    if A.dim() != 2 or B.dim() != 3:
+        raise ValueError(f"gemm_grouped takes A (rows x K) and B (groups x K x N), not {A.dim()}-D and {B.dim()}-D")
+    code = _dtype_code(A, "A", ("float16", "bfloat16", "uint8"))
+    (rows, K), dev = A.shape, A.device
+    N = B.shape[1] if b_transposed else B.shape[2]
+    groups = _groups(offsets, dev)
+    _need("B", B, (groups, N, K) if b_transposed else (groups, K, N), A.dtype, dev)
+    lda = _need("A", A, (rows, K), A.dtype, dev)
+    if row_scale is not None:
+        _need("row_scale", row_scale, (rows,), torch.float32, dev)
+    if group_scale is not None:
+        _need("group_scale", group_scale, (groups,), torch.float32, dev)
+    otype = _out_type(out_dtype)
+    with _scope(dev, stream):
+        if C is None:
+            C = torch.empty((rows, N), dtype=otype, device=dev)
+        ldc = _need("C", C, (rows, N), otype, dev)
+        _check(lib().bw_gemm_grouped(code, _ptr(A), lda, _ptr(B), int(b_transposed), _ptr(offsets), groups,
+                                     _ptr(row_scale), _ptr(group_scale), _ptr(C), ldc, out_dtype, rows, N, K,
+                                     _stream(None)))
+    return C
+
+
+def gemm_grouped_wgrad(X, Y, offsets, D=None, out_dtype=OUT_F32, stream=None):
+    """D[g] = X[rows of g]^T x Y[rows of g], zeros for a group without rows: the weight gradient of
+    gemm_grouped (X = A, Y = dC for a groups x K x N matrix; X = dC, Y = A for groups x N x K).
+    X: rows x M, Y: rows x N, both float16 or both bfloat16; D: groups x M x N."""
+    import torch
+
+    if X.dim() != 2 or Y.dim() != 2:
+        raise ValueError(f"gemm_grouped_wgrad takes X (rows x M) and Y (rows x N), not {X.dim()}-D and {Y.dim()}-D")
+    code = _dtype_code(X, "X", ("float16", "bfloat16"))
+    (rows, M), N, dev = X.shape, Y.shape[1], X.device
+    groups = _groups(offsets, dev)
+    ldx = _need("X", X, (rows, M), X.dtype, dev)
+    ldy = _need("Y", Y, (rows, N), X.dtype, dev)
+    otype = _out_type(out_dtype)
+    with _scope(dev, stream):
+        if D is None:
+            D = torch.empty((groups, M, N), dtype=otype, device=dev)
+        _need("D", D, (groups, M, N), otype, dev)
+        _check(lib().bw_gemm_grouped_wgrad(code, _ptr(X), ldx, _ptr(Y), ldy, _ptr(offsets), groups, _ptr(D),
+                                           out_dtype, rows, M, N, _stream(None)))
+    return D
 
 
 def unshard_columns(C_shardmajor, M: int, N: int, world: int, out=None, stream=None):

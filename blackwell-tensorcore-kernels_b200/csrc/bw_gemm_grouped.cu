@@ -1,0 +1,189 @@
+// Entry points of the products grouped by expert: argument checks, TMA descriptors, tile choice and
+// launch of the kernels in bw_gemm_grouped.cuh.
+#include "bw_gemm_grouped.cuh"
+
+#include "bw_runtime.cuh"
+
+namespace bw {
+namespace {
+
+constexpr int kMaxSmem = 232448;
+
+struct Operands {  // what the tensor maps are made of
+  const void* A;
+  const void* B;
+  long long lda, ldb;  // elements between rows of A (X) and, in WGRAD, Y
+};
+
+CUtensorMapDataType map_type(int dtype) {
+  return dtype == BW_DTYPE_FP8 ? CU_TENSOR_MAP_DATA_TYPE_UINT8
+         : dtype == BW_DTYPE_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+}
+
+// Tile rows that the output can have at most, and that it has when the rows spread evenly.
+long long max_tile_rows(int rows, int groups, int tm) {
+  return rows / tm + (groups < rows ? groups : rows);
+}
+long long even_tile_rows(int rows, int groups, int tm) {
+  const long long active = groups < rows ? groups : rows;
+  const long long each = (rows + active - 1) / active;
+  return active * ((each + tm - 1) / tm);
+}
+
+template <Kind KIND, GMode MODE, Out OUT>
+int launch(const Operands& o, int dtype, GroupedParams p, cudaStream_t s, const DeviceState& d) {
+  const bool wgrad = MODE == GMode::WGRAD;
+  const int es = dtype == BW_DTYPE_FP8 ? 1 : 2;
+  const CUtensorMapDataType ty = map_type(dtype);
+  const long long mt = wgrad ? static_cast<long long>(p.groups) * ((p.m + kBM - 1) / kBM) : even_tile_rows(p.rows, p.groups, kBM);
+  // the widest tile that still gives every SM one
+  p.W = 256;
+  while (p.W > 64 && mt * ((p.n + p.W - 1) / p.W) < d.sms) p.W /= 2;
+  const long long most = (wgrad ? mt : max_tile_rows(p.rows, p.groups, kBM)) * ((p.n + p.W - 1) / p.W);
+  if (most >= (1LL << 31) - 4096) return set_error(BW_ERR_INVALID, "grouped GEMM: %lld output tiles exceed the index range", most);
+  p.stage_bytes = (kBM + p.W) * kSlabBytes;
+  p.stages = (kMaxSmem - grouped_tail_bytes(p.groups)) / p.stage_bytes;
+  if (p.stages > kGroupedMaxStages) p.stages = kGroupedMaxStages;
+  CUtensorMap ta{}, tb{};
+  int r = BW_OK;
+  constexpr int KE = KindTraits<KIND>::kElemsPerSlab;
+  if ((wgrad ? p.rows : p.k) > 0) {
+    if (wgrad) {
+      r = make_tmap_2d(&ta, ty, o.A, p.m, p.rows, uint64_t(o.lda) * es, 64, 64);
+      if (r == BW_OK) r = make_tmap_2d(&tb, ty, o.B, p.n, p.rows, uint64_t(o.ldb) * es, 64, 64);
+    } else {
+      r = make_tmap_2d(&ta, ty, o.A, p.k, p.rows, uint64_t(o.lda) * es, KE, kBM);
+      if (r == BW_OK)
+        r = MODE == GMode::ROWS_NK
+                ? make_tmap_3d(&tb, ty, o.B, p.k, p.n, p.groups, uint64_t(p.k) * es, uint64_t(p.k) * p.n * es, KE, p.W)
+                : make_tmap_3d(&tb, ty, o.B, p.n, p.k, p.groups, uint64_t(p.n) * es, uint64_t(p.k) * p.n * es, 64, 64);
+    }
+    if (r != BW_OK) return r;
+  }
+  auto kern = bw_tc_gemm_grouped_kernel<KIND, MODE, OUT>;
+  static bool attr_done[64] = {};
+  int dev = 0;
+  BW_CUDA(cudaGetDevice(&dev));
+  if (!attr_done[dev & 63]) {
+    BW_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxSmem));
+    attr_done[dev & 63] = true;
+  }
+  const int grid = static_cast<int>(most < d.sms ? most : d.sms);
+  kern<<<grid, kGroupedThreads, p.stages * p.stage_bytes + grouped_tail_bytes(p.groups), s>>>(ta, tb, p);
+  BW_CUDA(cudaGetLastError());
+  return BW_OK;
+}
+
+template <Kind KIND, GMode MODE>
+int launch_out(const Operands& o, int dtype, int out_dtype, const GroupedParams& p, cudaStream_t s, const DeviceState& d) {
+  if (out_dtype == BW_OUT_F32) return launch<KIND, MODE, Out::F32>(o, dtype, p, s, d);
+  return launch<KIND, MODE, Out::BF16>(o, dtype, p, s, d);
+}
+
+int check_grouped(const char* name, int dtype, bool fp8, int out_dtype, const int* offsets, int groups, int rows, int a,
+                  int b) {
+  if (dtype != BW_DTYPE_F16 && dtype != BW_DTYPE_BF16 && !(fp8 && dtype == BW_DTYPE_FP8))
+    return set_error(BW_ERR_INVALID, "%s: bad dtype %d", name, dtype);
+  if (out_dtype != BW_OUT_F32 && out_dtype != BW_OUT_BF16)
+    return set_error(BW_ERR_INVALID, "%s: bad out_dtype %d", name, out_dtype);
+  if (rows < 0 || a < 0 || b < 0) return set_error(BW_ERR_INVALID, "%s: negative size", name);
+  if (groups < 1 || groups > kMaxGroups) return set_error(BW_ERR_INVALID, "%s: groups = %d (1..%d)", name, groups, kMaxGroups);
+  if (!offsets || (reinterpret_cast<uintptr_t>(offsets) & 3u))
+    return set_error(BW_ERR_INVALID, "%s: offsets is null or not aligned to an int", name);
+  return BW_OK;
+}
+
+int check_operand(const char* name, const char* what, const void* p, long long ld, long long rows, int cols, int es) {
+  if (!p) return set_error(BW_ERR_INVALID, "%s: %s is null", name, what);
+  if (ld < cols && rows > 1) return set_error(BW_ERR_INVALID, "%s: %s's row pitch %lld is below %d", name, what, ld, cols);
+  if (!aligned16(p) || (rows > 1 && ld * es % 16 != 0))
+    return set_error(BW_ERR_INVALID, "%s: %s and its row pitch must be multiples of 16 bytes", name, what);
+  return BW_OK;
+}
+
+// The widest store that every row of C allows.
+int store_width(const void* C, long long ldc, int elem) {
+  for (int w = 32; w >= 16; w /= 2)
+    if (reinterpret_cast<uintptr_t>(C) % w == 0 && ldc * elem % w == 0) return w;
+  return elem;
+}
+
+GroupedParams base(const DeviceState& d, int dtype, void* C, long long ldc, int out_dtype, const int* offsets, int groups,
+                   int rows) {
+  GroupedParams p{};
+  p.C = C;
+  p.ldc = ldc;
+  p.offsets = offsets;
+  p.groups = groups;
+  p.rows = rows;
+  p.group_m = 16;
+  p.vec = store_width(C, ldc, out_dtype == BW_OUT_F32 ? 4 : 2);
+  p.fmt = dtype == BW_DTYPE_BF16 ? 1u : 0u;  // kind::f16: 0 FP16, 1 BF16; kind::f8f6f4: 0 E4M3
+  p.status = d.status;
+  p.budget_ns = wait_budget_ns();
+  return p;
+}
+
+}  // namespace
+}  // namespace bw
+
+using namespace bw;
+
+extern "C" {
+
+int bw_gemm_grouped(int dtype, const void* A, long long lda, const void* B, int b_transposed, const int* offsets,
+                    int groups, const float* row_scale, const float* group_scale, void* C, long long ldc,
+                    int out_dtype, int rows, int N, int K, void* stream) {
+  const char* name = "grouped GEMM";
+  int r = check_grouped(name, dtype, true, out_dtype, offsets, groups, rows, N, K);
+  if (r != BW_OK) return r;
+  if (dtype == BW_DTYPE_FP8 && !b_transposed)
+    return set_error(BW_ERR_INVALID, "%s: E4M3 takes a K-contiguous B (b_transposed)", name);
+  if (rows == 0 || N == 0) return BW_OK;
+  const int oe = out_dtype == BW_OUT_F32 ? 4 : 2, es = dtype == BW_DTYPE_FP8 ? 1 : 2;
+  if (!C || reinterpret_cast<uintptr_t>(C) % oe) return set_error(BW_ERR_INVALID, "%s: C is null or not aligned to its element", name);
+  if (rows > 1 && ldc < N) return set_error(BW_ERR_INVALID, "%s: C's row pitch %lld is below N = %d", name, ldc, N);
+  if (((reinterpret_cast<uintptr_t>(row_scale) | reinterpret_cast<uintptr_t>(group_scale)) & 3u))
+    return set_error(BW_ERR_INVALID, "%s: scales are not aligned to a float", name);
+  if (rows == 1) { lda = (K + 15LL) / 16 * 16; ldc = ldc < N ? N : ldc; }  // a single row has no pitch
+  if (K > 0) {
+    if ((r = check_operand(name, "A", A, lda, rows, K, es)) != BW_OK) return r;
+    const int inner = b_transposed ? K : N;
+    if ((r = check_operand(name, "B", B, inner, 2, inner, es)) != BW_OK) return r;
+  }
+  DeviceState* d;
+  if ((r = ensure_device(&d)) != BW_OK) return r;
+  GroupedParams p = base(*d, dtype, C, ldc, out_dtype, offsets, groups, rows);
+  p.row_scale = row_scale;
+  p.group_scale = group_scale;
+  p.n = N;
+  p.k = K;
+  const Operands o{A, B, lda, 0};
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  if (dtype == BW_DTYPE_FP8) return launch_out<Kind::F8, GMode::ROWS_NK>(o, dtype, out_dtype, p, s, *d);
+  if (b_transposed) return launch_out<Kind::F16, GMode::ROWS_NK>(o, dtype, out_dtype, p, s, *d);
+  return launch_out<Kind::F16, GMode::ROWS_KN>(o, dtype, out_dtype, p, s, *d);
+}
+
+int bw_gemm_grouped_wgrad(int dtype, const void* X, long long ldx, const void* Y, long long ldy, const int* offsets,
+                          int groups, void* D, int out_dtype, int rows, int M, int N, void* stream) {
+  const char* name = "grouped weight gradient";
+  int r = check_grouped(name, dtype, false, out_dtype, offsets, groups, rows, M, N);
+  if (r != BW_OK) return r;
+  if (M == 0 || N == 0) return BW_OK;
+  const int oe = out_dtype == BW_OUT_F32 ? 4 : 2;
+  if (!D || reinterpret_cast<uintptr_t>(D) % oe) return set_error(BW_ERR_INVALID, "%s: D is null or not aligned to its element", name);
+  if (rows == 1) { ldx = (M + 7LL) / 8 * 8; ldy = (N + 7LL) / 8 * 8; }
+  if (rows > 0 && ((r = check_operand(name, "X", X, ldx, rows, M, 2)) != BW_OK ||
+                   (r = check_operand(name, "Y", Y, ldy, rows, N, 2)) != BW_OK))
+    return r;
+  DeviceState* d;
+  if ((r = ensure_device(&d)) != BW_OK) return r;
+  GroupedParams p = base(*d, dtype, D, N, out_dtype, offsets, groups, rows);
+  p.m = M;
+  p.n = N;
+  const Operands o{X, Y, ldx, ldy};
+  return launch_out<Kind::F16, GMode::WGRAD>(o, dtype, out_dtype, p, static_cast<cudaStream_t>(stream), *d);
+}
+
+}  // extern "C"

@@ -153,6 +153,26 @@ int make_tmap_2d(CUtensorMap* map, CUtensorMapDataType dtype, const void* base, 
   return BW_OK;
 }
 
+int make_tmap_3d(CUtensorMap* map, CUtensorMapDataType dtype, const void* base, uint64_t inner, uint64_t mid,
+                 uint64_t outer, uint64_t mid_stride_bytes, uint64_t outer_stride_bytes, uint32_t box_inner,
+                 uint32_t box_mid) {
+  int r = load_encode();
+  if (r != BW_OK) return r;
+  cuuint64_t dims[3] = {inner, mid, outer};
+  cuuint64_t strides[2] = {mid_stride_bytes, outer_stride_bytes};
+  cuuint32_t box[3] = {box_inner, box_mid, 1};
+  cuuint32_t estr[3] = {1, 1, 1};
+  CUresult cr = g_encode(map, dtype, 3, const_cast<void*>(base), dims, strides, box, estr,
+                         CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                         CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (cr != CUDA_SUCCESS)
+    return set_error(BW_ERR_CUDA, "cuTensorMapEncodeTiled failed (%d): dims %llu x %llu x %llu strides %llu, %llu",
+                     static_cast<int>(cr), (unsigned long long)inner, (unsigned long long)mid,
+                     (unsigned long long)outer, (unsigned long long)mid_stride_bytes,
+                     (unsigned long long)outer_stride_bytes);
+  return BW_OK;
+}
+
 }  // namespace bw
 
 using namespace bw;

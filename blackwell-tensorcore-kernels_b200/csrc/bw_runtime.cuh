@@ -49,6 +49,11 @@ int make_tmap_2d(CUtensorMap* map, CUtensorMapDataType dtype, const void* base, 
                  uint64_t row_stride_bytes, uint32_t box_inner, uint32_t box_outer,
                  CUtensorMapSwizzle swizzle = CU_TENSOR_MAP_SWIZZLE_128B);
 
+// 3-D row-major tensor map (dims {inner, mid, outer}, box {box_inner, box_mid, 1}), 128B swizzle.
+int make_tmap_3d(CUtensorMap* map, CUtensorMapDataType dtype, const void* base, uint64_t inner, uint64_t mid,
+                 uint64_t outer, uint64_t mid_stride_bytes, uint64_t outer_stride_bytes, uint32_t box_inner,
+                 uint32_t box_mid);
+
 // [world][M][N/world] -> row-major M x N for 4-byte (FP32) or 2-byte (BF16) elements.
 int unshard_elems(const void* src, void* dst, int M, int N, int world, int elem_bytes, cudaStream_t stream);
 

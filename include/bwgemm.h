@@ -184,6 +184,31 @@ int bw_rmsnorm_backward(const void* dy, long long lddy, const void* h, long long
                         long long lddx, float* dweight, void* workspace, size_t workspace_bytes, int rows, int cols,
                         void* stream);
 
+/* ---------------- products grouped by expert ---------------- */
+/* No counterpart in the reference. The rows of A that belong to group g, offsets[g] <= r <
+ * offsets[g + 1], are multiplied by matrix g of B:
+ *   C[r, :] = (sum_k A[r, k] B_g[k, :]) * row_scale[r] * group_scale[g]
+ * A: rows x K (pitch lda), C: rows x N (pitch ldc) in out_dtype (BW_OUT_F32 or BW_OUT_BF16), FP32 accumulation.
+ * dtype BW_DTYPE_F16 or BF16: B is groups x K x N, or with b_transposed groups x N x K; the two are
+ *   each other's input gradient (dA = grouped product of dC with the other layout of the same B).
+ * dtype BW_DTYPE_FP8: E4M3, b_transposed only (both operands K-contiguous).
+ * row_scale (one float a row) and group_scale (one a group) may be NULL: 1.
+ * offsets: groups + 1 ints in device memory, read by the kernel (no synchronisation; a captured
+ * graph replays with new sizes). Empty groups are allowed. Rows before offsets[0] and behind
+ * offsets[groups] are left as they were. Offsets outside 0..rows count as the nearest of the two, one below its
+ * predecessor as its predecessor. 1 <= groups <= 1024. K = 0 writes zeros.
+ * Alignment: A, B 16 bytes, as are lda, and B's rows (K or N elements); C its element (16- or
+ * 32-byte aligned rows store faster). */
+int bw_gemm_grouped(int dtype, const void* A, long long lda, const void* B, int b_transposed, const int* offsets,
+                    int groups, const float* row_scale, const float* group_scale, void* C, long long ldc,
+                    int out_dtype, int rows, int N, int K, void* stream);
+/* Weight gradient of the above: D[g] = X[rows of g]^T Y[rows of g], zeros for a group without rows.
+ * X: rows x M (pitch ldx), Y: rows x N (pitch ldy), dtype BW_DTYPE_F16 or BF16; D: groups x M x N in out_dtype.
+ * With X = A, Y = dC it is the gradient of a groups x K x N matrix, with X = dC, Y = A of its
+ * transposed form. Alignment: X, Y and their pitches 16 bytes, D its element. */
+int bw_gemm_grouped_wgrad(int dtype, const void* X, long long ldx, const void* Y, long long ldy, const int* offsets,
+                          int groups, void* D, int out_dtype, int rows, int M, int N, void* stream);
+
 /* ---------------- N-sharded multi-GPU GEMM helpers ---------------- */
 /* Column sharding (one process per GPU) needs no new GEMM: rank r calls bw_gemm_* on its
  * shard B[:, r*N/world:(r+1)*N/world]. When a gathered C is requested, the host layer
