@@ -292,78 +292,113 @@ def quantize_mxfp4(src, transpose=False, mode=MX_BLOCK32, dst=None, sf=None, str
     return dst, sf
 
 
-# ------------------------------------------------------------------ root-mean-square norm
-def _dtype_code(t, what: str, allowed: tuple[str, ...]) -> int:
-    import torch
+# ------------------------------------------------------------------ operands of the calls below
+# The wrappers below are called once or twice a layer on a few rows, where their own time counts:
+# checks compare without building anything, and outputs come from the cheapest allocation call.
+_type_codes = {}  # torch dtype -> (BW_DTYPE_*); filled on first use, torch being imported lazily
 
-    codes = {torch.float32: ("float32", DTYPE_F32), torch.float16: ("float16", DTYPE_F16),
-             torch.bfloat16: ("bfloat16", DTYPE_BF16), torch.uint8: ("uint8", DTYPE_FP8)}
-    name, code = codes.get(t.dtype, (str(t.dtype), -1))
-    if name not in allowed:
-        raise TypeError(f"{what} must be {' or '.join(allowed)}, not {name}")
+
+def _codes():
+    if not _type_codes:
+        import torch
+
+        _type_codes.update({torch.float32: DTYPE_F32, torch.float16: DTYPE_F16, torch.bfloat16: DTYPE_BF16,
+                             torch.uint8: DTYPE_FP8})
+    return _type_codes
+
+
+def _dtype_code(t, what: str, allowed: tuple[int, ...]) -> int:
+    code = _codes().get(t.dtype, -1)
+    if code not in allowed:
+        names = " or ".join(str(k) for k, v in _codes().items() if v in allowed)
+        raise TypeError(f"{what} must be {names}, not {t.dtype}")
     return code
 
 
-def _need(what: str, t, shape: tuple, dtype, device, pitched: bool = True) -> int:
-    """Checks an operand's shape, type, device and layout; returns the row pitch of a 2-D one."""
+def _refuse(what: str, t, shape, dtype, dev: int):
     if t.dtype != dtype:
         raise TypeError(f"{what} must be {dtype}, not {t.dtype}")
-    if tuple(t.shape) != shape:
-        raise ValueError(f"{what} has shape {tuple(t.shape)}, expected {shape}")
-    if t.device != device:
-        raise ValueError(f"{what} is on {t.device}, expected {device}")
-    if len(shape) == 2 and pitched:
-        if shape[1] > 1 and t.stride(1) != 1:
-            raise ValueError(f"{what} must have contiguous rows (strides {t.stride()})")
-        return t.stride(0) if shape[0] > 1 else shape[1]
-    if not t.is_contiguous():
-        raise ValueError(f"{what} must be contiguous")
-    return 0
+    if tuple(t.shape) != tuple(shape):
+        raise ValueError(f"{what} has shape {tuple(t.shape)}, expected {tuple(shape)}")
+    if t.get_device() != dev:
+        raise ValueError(f"{what} is on {t.device}, the other operands are on cuda:{dev}")
+    raise ValueError(f"{what} must be contiguous (strides {t.stride()})")
+
+
+def _rows(what: str, t, shape, dtype, dev: int) -> int:
+    """Row pitch of a 2-D operand with contiguous rows."""
+    if t.dtype is not dtype or t.shape != shape or t.get_device() != dev:
+        _refuse(what, t, shape, dtype, dev)
+    ld, step = t.stride()
+    if step != 1 and shape[1] > 1:
+        _refuse(what, t, shape, dtype, dev)
+    return ld if shape[0] > 1 else shape[1]
+
+
+def _flat(what: str, t, shape, dtype, dev: int) -> None:
+    if t.dtype is not dtype or t.shape != shape or t.get_device() != dev or not t.is_contiguous():
+        _refuse(what, t, shape, dtype, dev)
 
 
 _NO_SCOPE = contextlib.nullcontext()
 
 
-def _scope(device, stream):
-    """Makes `device` (the operands') and `stream` current: what a call allocates belongs to the
-    stream that it runs on."""
+def _scope(t, stream):
+    """Makes the operands' device and `stream` current: what a call allocates belongs to the stream
+    that it runs on."""
     import torch
 
-    if device.type != "cuda":
-        raise ValueError(f"operands must be on a CUDA device, not {device}")
+    dev = t.get_device()
+    if dev < 0:
+        raise ValueError(f"operands must be on a CUDA device, not {t.device}")
     if stream is None:
-        return _NO_SCOPE if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+        return _NO_SCOPE if dev == torch.cuda.current_device() else torch.cuda.device(dev)
     if isinstance(stream, int):
-        stream = torch.cuda.ExternalStream(stream, device=device)
-    if stream.device != device:
-        raise ValueError(f"stream is of {stream.device}, operands are on {device}")
+        stream = torch.cuda.ExternalStream(stream, device=dev)
+    if stream.device.index != dev:
+        raise ValueError(f"stream is of {stream.device}, operands are on cuda:{dev}")
     return torch.cuda.stream(stream)
+
+
+def _current_stream(dev: int) -> int:
+    import torch
+
+    raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)  # the handle alone, without a Stream object
+    return raw(dev) if raw is not None else torch.cuda.current_stream(dev).cuda_stream
+
+
+# ------------------------------------------------------------------ root-mean-square norm
+_NORM_TYPES = (DTYPE_F32, DTYPE_F16, DTYPE_BF16)
 
 
 def _norm_operands(x, weight, residual):
     if x.dim() != 2 or weight.dim() != 1:
         raise ValueError(f"rmsnorm takes x (rows x cols) and weight (cols), not {x.dim()}-D and {weight.dim()}-D")
-    code = _dtype_code(x, "x", ("float32", "float16", "bfloat16"))
-    shape, dev = tuple(x.shape), x.device
-    ldx = _need("x", x, shape, x.dtype, dev)
-    wcode = DTYPE_F32 if weight.dtype.itemsize == 4 else code
+    dtype, shape, dev = x.dtype, x.shape, x.get_device()
+    code = _dtype_code(x, "x", _NORM_TYPES)
+    wtype = weight.dtype
+    if wtype is not dtype and _codes().get(wtype) != DTYPE_F32:
+        raise TypeError(f"weight must be {dtype} or torch.float32, not {wtype}")
+    _flat("weight", weight, shape[1:], wtype, dev)
+    ldx = _rows("x", x, shape, dtype, dev)
+    ldr = _rows("residual", residual, shape, dtype, dev) if residual is not None else 0
+    return code, code if wtype is dtype else DTYPE_F32, dtype, shape, dev, ldx, ldr
+
+
+def _norm_outputs(x, shape, dtype, dev, residual, h, rstd):
+    """(h, its pitch, the h to be written or None, rstd)."""
     import torch
 
-    _need("weight", weight, (shape[1],), torch.float32 if wcode == DTYPE_F32 else x.dtype, dev)
-    ldr = _need("residual", residual, shape, x.dtype, dev) if residual is not None else 0
-    return code, wcode, shape, dev, ldx, ldr
-
-
-def _norm_outputs(x, shape, dev, residual, h, rstd):
-    import torch
-
-    if h is None:
-        h = torch.empty(shape, dtype=x.dtype, device=dev) if residual is not None else x
-    ldh = _need("h", h, shape, x.dtype, dev)
     if rstd is None:
-        rstd = torch.empty(shape[0], dtype=torch.float32, device=dev)
-    _need("rstd", rstd, (shape[0],), torch.float32, dev)
-    return h, ldh, rstd, None if h is x else h
+        rstd = torch.empty_strided((shape[0],), (1,), dtype=torch.float32, device=x.device)
+    else:
+        _flat("rstd", rstd, shape[:1], torch.float32, dev)
+    if h is None:
+        if residual is None:
+            return x, 0, None, rstd
+        h = torch.empty_strided(shape, (shape[1], 1), dtype=dtype, device=x.device)
+        return h, shape[1], h, rstd
+    return h, _rows("h", h, shape, dtype, dev), h, rstd
 
 
 def rmsnorm(x, weight, residual=None, eps: float = 1e-6, y=None, h=None, rstd=None, stream=None):
@@ -374,14 +409,15 @@ def rmsnorm(x, weight, residual=None, eps: float = 1e-6, y=None, h=None, rstd=No
     rmsnorm_backward takes. y and h may be x's or the residual's own tensor."""
     import torch
 
-    code, wcode, shape, dev, ldx, ldr = _norm_operands(x, weight, residual)
-    with _scope(dev, stream):
-        h, ldh, rstd, hout = _norm_outputs(x, shape, dev, residual, h, rstd)
+    code, wcode, dtype, shape, dev, ldx, ldr = _norm_operands(x, weight, residual)
+    with _scope(x, stream):
+        h, ldh, hout, rstd = _norm_outputs(x, shape, dtype, dev, residual, h, rstd)
         if y is None:
-            y = torch.empty(shape, dtype=x.dtype, device=dev)
-        ldy = _need("y", y, shape, x.dtype, dev)
-        _check(lib().bw_rmsnorm(_ptr(x), ldx, _ptr(residual), ldr, _ptr(weight), code, wcode, eps, _ptr(y), ldy,
-                                _ptr(hout), ldh, _ptr(rstd), shape[0], shape[1], _stream(None)))
+            y = torch.empty_strided(shape, (shape[1], 1), dtype=dtype, device=x.device)
+        ldy = _rows("y", y, shape, dtype, dev)
+        _check(lib().bw_rmsnorm(x.data_ptr(), ldx, _ptr(residual), ldr, weight.data_ptr(), code, wcode, eps,
+                                y.data_ptr(), ldy, _ptr(hout), ldh, rstd.data_ptr(), shape[0], shape[1],
+                                _current_stream(dev)))
     return y, h, rstd
 
 
@@ -390,17 +426,19 @@ def rmsnorm_fp8(x, weight, residual=None, eps: float = 1e-6, q=None, row_scale=N
     y = q * row_scale, as gemm_grouped takes them; returns (q, row_scale, h, rstd)."""
     import torch
 
-    code, wcode, shape, dev, ldx, ldr = _norm_operands(x, weight, residual)
-    with _scope(dev, stream):
-        h, ldh, rstd, hout = _norm_outputs(x, shape, dev, residual, h, rstd)
+    code, wcode, dtype, shape, dev, ldx, ldr = _norm_operands(x, weight, residual)
+    with _scope(x, stream):
+        h, ldh, hout, rstd = _norm_outputs(x, shape, dtype, dev, residual, h, rstd)
         if q is None:
-            q = torch.empty(shape, dtype=torch.uint8, device=dev)
-        ldq = _need("q", q, shape, torch.uint8, dev)
+            q = torch.empty_strided(shape, (shape[1], 1), dtype=torch.uint8, device=x.device)
+        ldq = _rows("q", q, shape, torch.uint8, dev)
         if row_scale is None:
-            row_scale = torch.empty(shape[0], dtype=torch.float32, device=dev)
-        _need("row_scale", row_scale, (shape[0],), torch.float32, dev)
-        _check(lib().bw_rmsnorm_fp8(_ptr(x), ldx, _ptr(residual), ldr, _ptr(weight), code, wcode, eps, _ptr(q), ldq,
-                                    _ptr(row_scale), _ptr(hout), ldh, _ptr(rstd), shape[0], shape[1], _stream(None)))
+            row_scale = torch.empty_strided((shape[0],), (1,), dtype=torch.float32, device=x.device)
+        else:
+            _flat("row_scale", row_scale, shape[:1], torch.float32, dev)
+        _check(lib().bw_rmsnorm_fp8(x.data_ptr(), ldx, _ptr(residual), ldr, weight.data_ptr(), code, wcode, eps,
+                                    q.data_ptr(), ldq, row_scale.data_ptr(), _ptr(hout), ldh, rstd.data_ptr(),
+                                    shape[0], shape[1], _current_stream(dev)))
     return q, row_scale, h, rstd
 
 
@@ -411,24 +449,27 @@ def rmsnorm_backward(dy, h, weight, rstd, dresidual=None, dx=None, dweight=None,
     bw_rmsnorm_backward_workspace(rows, cols) bytes; one of the call's own where None."""
     import torch
 
-    code, wcode, shape, dev, ldh, _ = _norm_operands(h, weight, None)
-    lddy = _need("dy", dy, shape, h.dtype, dev)
-    _need("rstd", rstd, (shape[0],), torch.float32, dev)
-    lddr = _need("dresidual", dresidual, shape, h.dtype, dev) if dresidual is not None else 0
-    with _scope(dev, stream):
+    code, wcode, dtype, shape, dev, ldh, lddr = _norm_operands(h, weight, dresidual)
+    lddy = _rows("dy", dy, shape, dtype, dev)
+    _flat("rstd", rstd, shape[:1], torch.float32, dev)
+    with _scope(h, stream):
         if dx is None:
-            dx = torch.empty(shape, dtype=h.dtype, device=dev)
-        lddx = _need("dx", dx, shape, h.dtype, dev)
+            dx = torch.empty_strided(shape, (shape[1], 1), dtype=dtype, device=h.device)
+        lddx = _rows("dx", dx, shape, dtype, dev)
         if dweight is None:
-            dweight = torch.empty(shape[1], dtype=torch.float32, device=dev)
-        _need("dweight", dweight, (shape[1],), torch.float32, dev)
+            dweight = torch.empty_strided((shape[1],), (1,), dtype=torch.float32, device=h.device)
+        else:
+            _flat("dweight", dweight, shape[1:], torch.float32, dev)
         if workspace is None:
-            workspace = torch.empty(lib().bw_rmsnorm_backward_workspace(*shape), dtype=torch.uint8, device=dev)
-        elif workspace.dtype != torch.uint8 or workspace.device != dev or not workspace.is_contiguous():
-            raise ValueError("workspace must be a contiguous uint8 tensor on the operands' device")
-        _check(lib().bw_rmsnorm_backward(_ptr(dy), lddy, _ptr(h), ldh, _ptr(weight), code, wcode, _ptr(rstd),
-                                         _ptr(dresidual), lddr, _ptr(dx), lddx, _ptr(dweight), _ptr(workspace),
-                                         workspace.numel(), shape[0], shape[1], _stream(None)))
+            nbytes = lib().bw_rmsnorm_backward_workspace(*shape)
+            workspace = torch.empty_strided((nbytes,), (1,), dtype=torch.uint8, device=h.device)
+        else:
+            nbytes = workspace.numel()
+            _flat("workspace", workspace, (nbytes,), torch.uint8, dev)
+        _check(lib().bw_rmsnorm_backward(dy.data_ptr(), lddy, h.data_ptr(), ldh, weight.data_ptr(), code, wcode,
+                                         rstd.data_ptr(), _ptr(dresidual), lddr, dx.data_ptr(), lddx,
+                                         dweight.data_ptr(), workspace.data_ptr(), nbytes, shape[0], shape[1],
+                                         _current_stream(dev)))
     return dx, dweight
 
 
@@ -436,17 +477,19 @@ def rmsnorm_backward(dy, h, weight, rstd, dresidual=None, dx=None, dweight=None,
 def _out_type(out_dtype: int):
     import torch
 
-    if out_dtype not in (OUT_F32, OUT_BF16):
-        raise ValueError(f"out_dtype must be OUT_F32 or OUT_BF16, not {out_dtype}")
-    return torch.bfloat16 if out_dtype == OUT_BF16 else torch.float32
+    if out_dtype == OUT_BF16:
+        return torch.bfloat16
+    if out_dtype == OUT_F32:
+        return torch.float32
+    raise ValueError(f"out_dtype must be OUT_F32 or OUT_BF16, not {out_dtype}")
 
 
-def _groups(offsets, dev) -> int:
+def _groups(offsets, dev: int) -> int:
     import torch
 
     if offsets.dim() != 1 or offsets.shape[0] < 2:
         raise ValueError(f"offsets must hold groups + 1 ints, not a tensor of shape {tuple(offsets.shape)}")
-    _need("offsets", offsets, tuple(offsets.shape), torch.int32, dev)
+    _flat("offsets", offsets, offsets.shape, torch.int32, dev)
     return offsets.shape[0] - 1
 
 
@@ -462,24 +505,24 @@ def gemm_grouped(A, B, offsets, C=None, b_transposed: bool = False, row_scale=No
 
     if A.dim() != 2 or B.dim() != 3:
         raise ValueError(f"gemm_grouped takes A (rows x K) and B (groups x K x N), not {A.dim()}-D and {B.dim()}-D")
-    code = _dtype_code(A, "A", ("float16", "bfloat16", "uint8"))
-    (rows, K), dev = A.shape, A.device
+    code = _dtype_code(A, "A", (DTYPE_F16, DTYPE_BF16, DTYPE_FP8))
+    (rows, K), dev = A.shape, A.get_device()
     N = B.shape[1] if b_transposed else B.shape[2]
     groups = _groups(offsets, dev)
-    _need("B", B, (groups, N, K) if b_transposed else (groups, K, N), A.dtype, dev)
-    lda = _need("A", A, (rows, K), A.dtype, dev)
+    _flat("B", B, (groups, N, K) if b_transposed else (groups, K, N), A.dtype, dev)
+    lda = _rows("A", A, A.shape, A.dtype, dev)
     if row_scale is not None:
-        _need("row_scale", row_scale, (rows,), torch.float32, dev)
+        _flat("row_scale", row_scale, (rows,), torch.float32, dev)
     if group_scale is not None:
-        _need("group_scale", group_scale, (groups,), torch.float32, dev)
+        _flat("group_scale", group_scale, (groups,), torch.float32, dev)
     otype = _out_type(out_dtype)
-    with _scope(dev, stream):
+    with _scope(A, stream):
         if C is None:
-            C = torch.empty((rows, N), dtype=otype, device=dev)
-        ldc = _need("C", C, (rows, N), otype, dev)
-        _check(lib().bw_gemm_grouped(code, _ptr(A), lda, _ptr(B), int(b_transposed), _ptr(offsets), groups,
-                                     _ptr(row_scale), _ptr(group_scale), _ptr(C), ldc, out_dtype, rows, N, K,
-                                     _stream(None)))
+            C = torch.empty_strided((rows, N), (N, 1), dtype=otype, device=A.device)
+        ldc = _rows("C", C, (rows, N), otype, dev)
+        _check(lib().bw_gemm_grouped(code, A.data_ptr(), lda, B.data_ptr(), int(b_transposed), offsets.data_ptr(),
+                                     groups, _ptr(row_scale), _ptr(group_scale), C.data_ptr(), ldc, out_dtype, rows,
+                                     N, K, _current_stream(dev)))
     return C
 
 
@@ -491,18 +534,18 @@ def gemm_grouped_wgrad(X, Y, offsets, D=None, out_dtype=OUT_F32, stream=None):
 
     if X.dim() != 2 or Y.dim() != 2:
         raise ValueError(f"gemm_grouped_wgrad takes X (rows x M) and Y (rows x N), not {X.dim()}-D and {Y.dim()}-D")
-    code = _dtype_code(X, "X", ("float16", "bfloat16"))
-    (rows, M), N, dev = X.shape, Y.shape[1], X.device
+    code = _dtype_code(X, "X", (DTYPE_F16, DTYPE_BF16))
+    (rows, M), N, dev = X.shape, Y.shape[1], X.get_device()
     groups = _groups(offsets, dev)
-    ldx = _need("X", X, (rows, M), X.dtype, dev)
-    ldy = _need("Y", Y, (rows, N), X.dtype, dev)
+    ldx = _rows("X", X, X.shape, X.dtype, dev)
+    ldy = _rows("Y", Y, (rows, N), X.dtype, dev)
     otype = _out_type(out_dtype)
-    with _scope(dev, stream):
+    with _scope(X, stream):
         if D is None:
-            D = torch.empty((groups, M, N), dtype=otype, device=dev)
-        _need("D", D, (groups, M, N), otype, dev)
-        _check(lib().bw_gemm_grouped_wgrad(code, _ptr(X), ldx, _ptr(Y), ldy, _ptr(offsets), groups, _ptr(D),
-                                           out_dtype, rows, M, N, _stream(None)))
+            D = torch.empty_strided((groups, M, N), (M * N, N, 1), dtype=otype, device=X.device)
+        _flat("D", D, (groups, M, N), otype, dev)
+        _check(lib().bw_gemm_grouped_wgrad(code, X.data_ptr(), ldx, Y.data_ptr(), ldy, offsets.data_ptr(), groups,
+                                           D.data_ptr(), out_dtype, rows, M, N, _current_stream(dev)))
     return D
 
 

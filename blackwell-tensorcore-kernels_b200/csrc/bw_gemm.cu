@@ -1,7 +1,5 @@
 // GEMM entry points of the C ABI: argument checks, TMA descriptors, tile-shape choice and
 // launch of the persistent tcgen05 kernel (bw_gemm_kernel.cuh).
-#include <cstdlib>
-
 #include "bw_gemm_kernel.cuh"
 #include "bw_gemm_pair.cuh"
 #include "bw_gemm_pair_mx.cuh"
@@ -11,12 +9,6 @@
 
 namespace bw {
 namespace {
-
-int env_int(const char* name, int dflt) {
-  const char* s = getenv(name);
-  if (!s || !*s) return dflt;
-  return atoi(s);
-}
 
 template <Kind KIND, bool B_MN, int BN, int STAGES, int ACC_BUFS, Out OUT>
 int launch(const CUtensorMap& ta, const CUtensorMap& tb, const CUtensorMap& tc, GemmParams p, cudaStream_t stream,
@@ -38,29 +30,6 @@ int launch(const CUtensorMap& ta, const CUtensorMap& tb, const CUtensorMap& tc, 
   kern<<<grid, kThreads, Cfg::kSmemBytes, stream>>>(ta, tb, tc, p);
   BW_CUDA(cudaGetLastError());
   return BW_OK;
-}
-
-// Co-resident CTA pairs of a persistent `__cluster_dims__(2,1,1)` kernel (clusters must fit
-// inside one GPC, so this can be below sms / 2); falls back to sms / 2 if the query fails.
-template <typename Kernel>
-int pair_clusters_resident(Kernel kern, int threads, int smem_bytes, const DeviceState& d) {
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(2 * (d.sms / 2), 1, 1);
-  cfg.blockDim = dim3(threads, 1, 1);
-  cfg.dynamicSmemBytes = smem_bytes;
-  cudaLaunchAttribute attr;
-  attr.id = cudaLaunchAttributeClusterDimension;
-  attr.val.clusterDim.x = 2;
-  attr.val.clusterDim.y = 1;
-  attr.val.clusterDim.z = 1;
-  cfg.attrs = &attr;
-  cfg.numAttrs = 1;
-  int n = 0;
-  if (cudaOccupancyMaxActiveClusters(&n, kern, &cfg) != cudaSuccess || n <= 0) {
-    cudaGetLastError();
-    n = d.sms / 2;
-  }
-  return n;
 }
 
 template <Kind KIND, bool B_MN, int STAGES, Out OUT, bool DIRECT_EPI, int KSUB, int TN = 256, int EPI_BUFS = 2>

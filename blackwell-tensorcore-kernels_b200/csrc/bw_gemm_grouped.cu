@@ -1,7 +1,6 @@
 // Entry points of the products grouped by expert: argument checks, TMA descriptors, tile choice and
 // launch of the kernels in bw_gemm_grouped.cuh.
 #include "bw_gemm_grouped.cuh"
-
 #include "bw_runtime.cuh"
 
 namespace bw {
@@ -30,46 +29,90 @@ long long even_tile_rows(int rows, int groups, int tm) {
   return active * ((each + tm - 1) / tm);
 }
 
+// CTA pairs with 256 x 256 tiles where the groups have rows enough to fill them.
+bool use_pair(const GroupedParams& p, bool wgrad, const DeviceState& d) {
+  const int forced = env_int("BW_GROUPED_PAIR", -1);
+  if (forced >= 0) return forced != 0;
+  const long long tn = (p.n + 255) / 256;
+  const long long active = p.groups < p.rows ? p.groups : p.rows;
+  if (wgrad) return active > 0 && p.rows / active >= 256 && p.groups * ((p.m + 255LL) / 256) * tn >= d.sms / 2;
+  return p.rows / active >= 192 && even_tile_rows(p.rows, p.groups, 256) * tn >= d.sms / 2;
+}
+
+// Tile width of the single-CTA kernel: the multiple of `gran` from 64 to 256 with the least work on the
+// busiest SM, ceil(tiles / SMs) x (W + c): a tile reads W columns of B and (in c) its rows of A, and
+// costs a start and an end. Ties go to the wider tile. 8 tokens' rows over 8 matrices of 4096 x 2048
+// E4M3: W = 240 (144 tiles, one wave).
+int tile_width(const GroupedParams& p, long long tile_rows, int gran, bool wgrad, const DeviceState& d) {
+  const int forced = env_int("BW_GROUPED_W", 0);
+  if (forced >= 64 && forced <= 256 && forced % gran == 0) return forced;
+  const long long active = p.groups < p.rows ? p.groups : p.rows;
+  const long long each = wgrad || active == 0 ? kBM : p.rows / active;
+  const long long c = 32 + (each < kBM ? each : kBM);
+  long long best = -1;
+  int W = 64;
+  for (int w = 64; w <= 256; w += gran) {
+    const long long tiles = tile_rows * ((p.n + w - 1) / w);
+    const long long cost = (tiles + d.sms - 1) / d.sms * (w + c);
+    if (best < 0 || cost <= best) {
+      best = cost;
+      W = w;
+    }
+  }
+  return W;
+}
+
 template <Kind KIND, GMode MODE, Out OUT>
 int launch(const Operands& o, int dtype, GroupedParams p, cudaStream_t s, const DeviceState& d) {
-  const bool wgrad = MODE == GMode::WGRAD;
-  const int es = dtype == BW_DTYPE_FP8 ? 1 : 2;
-  const CUtensorMapDataType ty = map_type(dtype);
-  const long long mt = wgrad ? static_cast<long long>(p.groups) * ((p.m + kBM - 1) / kBM) : even_tile_rows(p.rows, p.groups, kBM);
-  // the widest tile that still gives every SM one
-  p.W = 256;
-  while (p.W > 64 && mt * ((p.n + p.W - 1) / p.W) < d.sms) p.W /= 2;
-  const long long most = (wgrad ? mt : max_tile_rows(p.rows, p.groups, kBM)) * ((p.n + p.W - 1) / p.W);
-  if (most >= (1LL << 31) - 4096) return set_error(BW_ERR_INVALID, "grouped GEMM: %lld output tiles exceed the index range", most);
-  p.stage_bytes = (kBM + p.W) * kSlabBytes;
-  p.stages = (kMaxSmem - grouped_tail_bytes(p.groups)) / p.stage_bytes;
-  if (p.stages > kGroupedMaxStages) p.stages = kGroupedMaxStages;
-  CUtensorMap ta{}, tb{};
-  int r = BW_OK;
+  constexpr bool wgrad = MODE == GMode::WGRAD;
   constexpr int KE = KindTraits<KIND>::kElemsPerSlab;
+  const int es = dtype == BW_DTYPE_FP8 ? 1 : 2;
+  const bool pair = use_pair(p, wgrad, d);
+  const int tm = pair ? 256 : kBM;
+  const long long mt = wgrad ? static_cast<long long>(p.groups) * ((p.m + tm - 1) / tm) : even_tile_rows(p.rows, p.groups, tm);
+  p.W = pair ? 256 : tile_width(p, mt, MODE == GMode::ROWS_NK ? 16 : 64, wgrad, d);
+  const long long most = (wgrad ? mt : max_tile_rows(p.rows, p.groups, tm)) * ((p.n + p.W - 1) / p.W);
+  if (most >= (1LL << 31) - 4096) return set_error(BW_ERR_INVALID, "grouped GEMM: %lld output tiles exceed the index range", most);
+  p.stage_bytes = pair ? kPairStageBytes : (kBM + p.W) * kSlabBytes;
+  p.stages = pair ? kPairStages : (kMaxSmem - grouped_tail_bytes(p.groups)) / p.stage_bytes;
+  if (p.stages > kGroupedMaxStages) p.stages = kGroupedMaxStages;
+  const int smem = p.stages * p.stage_bytes + grouped_tail_bytes(p.groups);
+  CUtensorMap ta{}, ta16{}, tb{};
   if ((wgrad ? p.rows : p.k) > 0) {
+    const CUtensorMapDataType ty = map_type(dtype);
+    const int b_box = pair ? 128 : p.W;  // a CTA of a pair loads its half of the tile's columns
+    int r;
     if (wgrad) {
       r = make_tmap_2d(&ta, ty, o.A, p.m, p.rows, uint64_t(o.lda) * es, 64, 64);
       if (r == BW_OK) r = make_tmap_2d(&tb, ty, o.B, p.n, p.rows, uint64_t(o.ldb) * es, 64, 64);
     } else {
       r = make_tmap_2d(&ta, ty, o.A, p.k, p.rows, uint64_t(o.lda) * es, KE, kBM);
+      if (r == BW_OK) r = make_tmap_2d(&ta16, ty, o.A, p.k, p.rows, uint64_t(o.lda) * es, KE, 16);
+      const uint64_t matrix = uint64_t(p.k) * p.n * es;
       if (r == BW_OK)
-        r = MODE == GMode::ROWS_NK
-                ? make_tmap_3d(&tb, ty, o.B, p.k, p.n, p.groups, uint64_t(p.k) * es, uint64_t(p.k) * p.n * es, KE, p.W)
-                : make_tmap_3d(&tb, ty, o.B, p.n, p.k, p.groups, uint64_t(p.n) * es, uint64_t(p.k) * p.n * es, 64, 64);
+        r = MODE == GMode::ROWS_NK ? make_tmap_3d(&tb, ty, o.B, p.k, p.n, p.groups, uint64_t(p.k) * es, matrix, KE, b_box)
+                                   : make_tmap_3d(&tb, ty, o.B, p.n, p.k, p.groups, uint64_t(p.n) * es, matrix, 64, 64);
     }
     if (r != BW_OK) return r;
   }
-  auto kern = bw_tc_gemm_grouped_kernel<KIND, MODE, OUT>;
-  static bool attr_done[64] = {};
   int dev = 0;
   BW_CUDA(cudaGetDevice(&dev));
-  if (!attr_done[dev & 63]) {
-    BW_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxSmem));
-    attr_done[dev & 63] = true;
+  auto one = bw_tc_gemm_grouped_kernel<KIND, MODE, OUT>;
+  auto two = bw_tc_gemm_grouped_pair_kernel<KIND, MODE, OUT>;
+  static int clusters[64] = {};  // co-resident CTA pairs; 0: kernels not set up on this device
+  if (clusters[dev & 63] == 0) {
+    BW_CUDA(cudaFuncSetAttribute(one, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxSmem));
+    BW_CUDA(cudaFuncSetAttribute(two, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxSmem));
+    clusters[dev & 63] = pair_clusters_resident(
+        two, kGroupedThreads, kPairStages * kPairStageBytes + grouped_tail_bytes(kMaxGroups), d);
   }
-  const int grid = static_cast<int>(most < d.sms ? most : d.sms);
-  kern<<<grid, kGroupedThreads, p.stages * p.stage_bytes + grouped_tail_bytes(p.groups), s>>>(ta, tb, p);
+  if (pair) {
+    const int n = static_cast<int>(most < clusters[dev & 63] ? most : clusters[dev & 63]);
+    two<<<2 * n, kGroupedThreads, smem, s>>>(ta, ta16, tb, p);
+  } else {
+    const int n = static_cast<int>(most < d.sms ? most : d.sms);
+    one<<<n, kGroupedThreads, smem, s>>>(ta, ta16, tb, p);
+  }
   BW_CUDA(cudaGetLastError());
   return BW_OK;
 }
@@ -103,9 +146,7 @@ int check_operand(const char* name, const char* what, const void* p, long long l
 
 // The widest store that every row of C allows.
 int store_width(const void* C, long long ldc, int elem) {
-  for (int w = 32; w >= 16; w /= 2)
-    if (reinterpret_cast<uintptr_t>(C) % w == 0 && ldc * elem % w == 0) return w;
-  return elem;
+  return aligned16(C) && ldc * elem % 16 == 0 ? 16 : elem;
 }
 
 GroupedParams base(const DeviceState& d, int dtype, void* C, long long ldc, int out_dtype, const int* offsets, int groups,

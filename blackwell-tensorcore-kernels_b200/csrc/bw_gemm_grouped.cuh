@@ -38,11 +38,24 @@ struct GroupedParams {
   int W;                     // tile width
   int stages, stage_bytes;
   int group_m;               // raster: tile rows a band
-  int vec;                   // store width in bytes: 32, 16, or the element's
+  int vec;                   // store width in bytes: 16, or the element's
   uint32_t fmt;              // operand format of the instruction descriptor
   int* status;
   unsigned long long budget_ns;
 };
+
+// One lane of a converged warp. elect.sync (not a comparison of the lane index) tells the compiler
+// that a single thread runs what follows, which tcgen05 and TMA instructions with their uniform
+// operands need to be issued without a loop over lanes.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "elect.sync _|p, 0xffffffff;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok));
+  return ok != 0;
+}
 
 // 3-D TMA load (no multicast).
 __device__ __forceinline__ void tma_load_3d(const CUtensorMap* m, uint64_t* bar, void* dst, int x, int y, int z,
@@ -54,10 +67,20 @@ __device__ __forceinline__ void tma_load_3d(const CUtensorMap* m, uint64_t* bar,
       : "memory");
 }
 
-// mbar_wait by a whole warp with one answer for all its lanes, so that a timeout takes the warp
+// Bounded wait like mbar_wait, which reads the global timer as soon as its first try fails; that read
+// takes longer than the wait of a running pipeline, so the timer starts after 64 tries here.
+__device__ __forceinline__ bool mbar_poll(uint64_t* bar, uint32_t parity, const WaitCtl& w, int where) {
+  const uint32_t a = smem_u32(bar);
+#pragma unroll 1
+  for (int i = 0; i < 64; ++i)
+    if (mbar_try_wait(a, parity)) return true;
+  return mbar_wait(bar, parity, w, where);
+}
+
+// The same by a whole warp with one answer for all its lanes, so that a timeout takes the warp
 // out of its loop together.
 __device__ __forceinline__ bool mbar_wait_warp(uint64_t* bar, uint32_t parity, const WaitCtl& w, int where) {
-  return __all_sync(0xffffffffu, mbar_wait(bar, parity, w, where));
+  return __all_sync(0xffffffffu, mbar_poll(bar, parity, w, where));
 }
 
 // Waits for a load of this CTA's own that is still in flight when a timeout ends the kernel early.
@@ -70,39 +93,36 @@ __device__ __forceinline__ void mbar_drain(uint64_t* bar, uint32_t parity, uint6
 
 // bounds[g] = first row of group g (bounds[groups] = end of the last), clamped and made
 // non-decreasing; tiles[g] = output tiles of the groups before g, `per_row` of them per tm rows.
-// Executed by one warp.
-__device__ __forceinline__ void grouped_schedule(const int* offsets, int groups, int rows, int tm, int per_row,
-                                                 int* bounds, int* tiles) {
+// All threads fetch the offsets (one trip to memory); warp 2 scans them.
+__device__ __forceinline__ void grouped_fetch(const int* offsets, int groups, int rows, int* bounds) {
+  for (int g = threadIdx.x; g <= groups; g += kGroupedThreads) bounds[g] = min(max(__ldg(offsets + g), 0), rows);
+}
+__device__ __forceinline__ void grouped_scan(int groups, int tm, int per_row, int* bounds, int* tiles) {
   const int lane = threadIdx.x & 31;
-  int high = 0;
+  int high = 0, sum = 0;
   for (int base = 0; base <= groups; base += 32) {
     const int g = base + lane;
-    int v = g <= groups ? min(max(__ldg(offsets + g), 0), rows) : 0;
+    int v = g <= groups ? bounds[g] : 0;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
       const int u = __shfl_up_sync(0xffffffffu, v, o);
       if (lane >= o) v = max(v, u);
     }
     v = max(v, high);
-    if (g <= groups) bounds[g] = v;
+    int before = __shfl_up_sync(0xffffffffu, v, 1);  // bounds[g - 1]
+    if (lane == 0) before = high;
     high = __shfl_sync(0xffffffffu, v, 31);
-  }
-  if (tiles == nullptr) return;
-  __syncwarp();
-  int sum = 0;
-  for (int base = 0; base < groups; base += 32) {
-    const int g = base + lane;
-    int v = g < groups ? (bounds[g + 1] - bounds[g] + tm - 1) / tm * per_row : 0;
-    const int own = v;
+    if (g <= groups) bounds[g] = v;
+    if (tiles == nullptr) continue;
+    int n = g > 0 && g <= groups ? (v - before + tm - 1) / tm * per_row : 0;  // tiles of group g - 1
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-      const int u = __shfl_up_sync(0xffffffffu, v, o);
-      if (lane >= o) v += u;
+      const int u = __shfl_up_sync(0xffffffffu, n, o);
+      if (lane >= o) n += u;
     }
-    if (g < groups) tiles[g] = sum + v - own;
-    sum += __shfl_sync(0xffffffffu, v, 31);
+    if (g <= groups) tiles[g] = sum + n;
+    sum += __shfl_sync(0xffffffffu, n, 31);
   }
-  if (lane == 0) tiles[groups] = sum;
 }
 
 // One output tile: its group, first output row and column, output rows that exist (ROWS_*: of the
@@ -153,107 +173,125 @@ struct GWalk {
   }
 };
 
-// Stores up to 32 columns of one row; `vec` bytes at a time where all of them exist.
-template <Out OUT>
-__device__ __forceinline__ void store_cols(void* base, long long at, const uint32_t (&r)[32], float alpha, int ncols,
-                                           int vec) {
-  if constexpr (OUT == Out::F32) {
-    float* dst = static_cast<float*>(base) + at;
-    if (vec >= 16 && ncols >= 32) {
-#pragma unroll
-      for (int g = 0; g < 4; ++g) {
-        uint32_t v[8];
-#pragma unroll
-        for (int j = 0; j < 8; ++j) v[j] = __float_as_uint(__uint_as_float(r[8 * g + j]) * alpha);
-        if (vec == 32) {
-          st_global_v8(dst + 8 * g, v);
-        } else {
-          st_global_v4(dst + 8 * g, make_uint4(v[0], v[1], v[2], v[3]));
-          st_global_v4(dst + 8 * g + 4, make_uint4(v[4], v[5], v[6], v[7]));
-        }
-      }
-    } else {
-#pragma unroll
-      for (int j = 0; j < 32; ++j)
-        if (j < ncols) dst[j] = __uint_as_float(r[j]) * alpha;
-    }
-  } else {
-    __nv_bfloat16* dst = static_cast<__nv_bfloat16*>(base) + at;
-    if (vec >= 16 && ncols >= 32) {
-#pragma unroll
-      for (int g = 0; g < 2; ++g) {
-        uint32_t v[8];
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          const __nv_bfloat162 h = __floats2bfloat162_rn(__uint_as_float(r[16 * g + 2 * j]) * alpha,
-                                                         __uint_as_float(r[16 * g + 2 * j + 1]) * alpha);
-          v[j] = *reinterpret_cast<const uint32_t*>(&h);
-        }
-        if (vec == 32) {
-          st_global_v8(dst + 16 * g, v);
-        } else {
-          st_global_v4(dst + 16 * g, make_uint4(v[0], v[1], v[2], v[3]));
-          st_global_v4(dst + 16 * g + 8, make_uint4(v[4], v[5], v[6], v[7]));
-        }
-      }
-    } else {
-#pragma unroll
-      for (int j = 0; j < 32; ++j)
-        if (j < ncols) dst[j] = __float2bfloat16_rn(__uint_as_float(r[j]) * alpha);
-    }
-  }
-}
-
-// One warp's 32 rows x W columns of a finished accumulator (zeros where nothing was summed).
-// `release` runs after the last read of the accumulator.
+// One warp's 32 rows x W columns of a finished accumulator (zeros where nothing was summed), 128
+// bytes of every row at a time: registers -> the warp's 4 KB of shared memory (16-byte pieces,
+// XOR-swizzled over the banks) -> 8 lanes a row, so that a store instruction covers whole 128-byte
+// lines. A lane storing its own row straight from registers touches 32 lines an instruction; tiles
+// that sum little (a gradient of few rows a group) are bound by that. `release` runs after the last
+// read of the accumulator.
 template <GMode MODE, Out OUT, typename Release>
 __device__ __forceinline__ void grouped_epilogue(const GroupedParams& p, const GTile& t, uint32_t tbase, int first,
-                                                 int lane, Release release) {
+                                                 int lane, uint32_t stage, Release release) {
+  constexpr int kCols = OUT == Out::F32 ? 32 : 64;     // columns in 128 bytes
+  constexpr int kElem = OUT == Out::F32 ? 4 : 2;
+  constexpr int kPiece = 16 / kElem;
   if (first >= t.rows) {  // none of this warp's rows exists
     release();
     return;
   }
-  const int r = first + lane;
-  const bool live = r < t.rows;
-  long long at;
+  const int nrows = min(32, t.rows - first);
+  long long row;
   float alpha = 1.f;
   if constexpr (MODE == GMode::WGRAD) {
-    at = (static_cast<long long>(t.g) * p.m + t.row0 + r) * p.ldc + t.col0;
+    row = static_cast<long long>(t.g) * p.m + t.row0 + first;
   } else {
-    at = static_cast<long long>(t.row0 + r) * p.ldc + t.col0;
-    if (p.group_scale && t.k > 0) alpha *= __ldg(p.group_scale + t.g);
-    if (p.row_scale && t.k > 0 && live) alpha *= __ldg(p.row_scale + t.row0 + r);
-  }
-  const int width = min(p.W, p.n - t.col0);
-#pragma unroll 1
-  for (int c = 0; c < width; c += 32) {
-    uint32_t v[32];
+    row = t.row0 + first;
     if (t.k > 0) {
-      tmem_ld_32x32b_x32(tbase + c, v);
-      tmem_ld_wait();
-      if (c + 32 >= width) release();
-    } else {
-#pragma unroll
-      for (int j = 0; j < 32; ++j) v[j] = 0;
+      if (p.group_scale) alpha *= __ldg(p.group_scale + t.g);
+      if (p.row_scale && lane < nrows) alpha *= __ldg(p.row_scale + row + lane);
     }
-    if (live) store_cols<OUT>(p.C, at + c, v, alpha, width - c, p.vec);
+  }
+  const long long pitch = p.ldc * kElem;
+  char* out = static_cast<char*>(p.C) + row * pitch + static_cast<long long>(t.col0) * kElem;
+  const int width = min(p.W, p.n - t.col0);
+  const bool summed = t.k > 0;
+  // the pieces that this lane stores: row rr + 4 i, piece jj (rows 4 apart alternate between two
+  // places of the swizzle)
+  const int rr = lane >> 3, jj = lane & 7;
+  const uint32_t from0 = stage + rr * 128 + ((jj ^ rr) << 4), from1 = stage + (rr + 4) * 128 + ((jj ^ (rr + 4)) << 4);
+  uint32_t v[kCols];
+  auto load = [&](int c) {
+    tmem_ld_32x32b_x32(tbase + c, *reinterpret_cast<uint32_t(*)[32]>(&v[0]));
+    if constexpr (kCols == 64) tmem_ld_32x32b_x32(tbase + c + 32, *reinterpret_cast<uint32_t(*)[32]>(&v[32]));
+  };
+  if (summed) load(0);
+#pragma unroll 1
+  for (int c = 0; c < width; c += kCols) {
+    uint32_t w[32];
+    if (summed) tmem_ld_wait();
+#pragma unroll
+    for (int j = 0; j < 32; ++j) {
+      if constexpr (OUT == Out::F32) {
+        w[j] = __float_as_uint(__uint_as_float(v[j]) * alpha);
+      } else {
+        const __nv_bfloat162 two =
+            __floats2bfloat162_rn(__uint_as_float(v[2 * j]) * alpha, __uint_as_float(v[2 * j + 1]) * alpha);
+        w[j] = *reinterpret_cast<const uint32_t*>(&two);
+      }
+      if (!summed) w[j] = 0;
+    }
+    if (summed) {  // the next columns come while these are stored
+      if (c + kCols < width) load(c + kCols);
+      else release();
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      st_shared_v4(stage + lane * 128 + ((j ^ (lane & 7)) << 4), w[4 * j], w[4 * j + 1], w[4 * j + 2], w[4 * j + 3]);
+    __syncwarp();
+    const int have = width - c - jj * kPiece;  // columns of this lane's pieces that exist
+    char* dst = out + rr * pitch + (c + jj * kPiece) * kElem;
+    if (p.vec == 16 && width - c >= kCols) {
+      uint4 x[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) x[i] = ld_shared_v4((i & 1 ? from1 : from0) + (i >> 1) * 1024);
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (rr + 4 * i < nrows) st_global_v4(dst + 4 * i * pitch, x[i]);
+    } else {
+#pragma unroll 1
+      for (int i = 0; i < 8; ++i) {
+        if (rr + 4 * i >= nrows || have <= 0) continue;
+        const uint4 x = ld_shared_v4((i & 1 ? from1 : from0) + (i >> 1) * 1024);
+        char* at = dst + 4 * i * pitch;
+        if (p.vec == 16 && have >= kPiece) {
+          st_global_v4(at, x);
+        } else {
+          const uint32_t e[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+          for (int k = 0; k < kPiece; ++k) {
+            if (k >= have) break;
+            if constexpr (OUT == Out::F32) reinterpret_cast<uint32_t*>(at)[k] = e[k];
+            else reinterpret_cast<uint16_t*>(at)[k] = static_cast<uint16_t>(e[k / 2] >> (16 * (k & 1)));
+          }
+        }
+      }
+    }
+    __syncwarp();
   }
 }
 
 __host__ __device__ constexpr int grouped_tail_bytes(int groups) {
   // barriers (full, empty, tailfull, fixed per stage; accfull, accempty x 2; teardown), TMEM slot and abort
-  // flag, bounds and tiles, alignment slack
-  return (4 * kGroupedMaxStages + 5) * 8 + 16 + 2 * (groups + 1) * 4 + 1024;
+  // flag, bounds and tiles, the epilogue's staging, alignment slack
+  return (4 * kGroupedMaxStages + 5) * 8 + 16 + 2 * (groups + 1) * 4 + kEpiWarps * kEpiBufBytes + 1024;
+}
+
+// A tile of few rows loads them in boxes of 16 (a box of 128 rows would fetch its neighbours' too, and
+// one that lies mostly behind the tensor's end is slow: 8 rows of 4096 x 2048 E4M3 times 8
+// matrices took 66 us with it, 19 us without).
+constexpr int kFewRows = 64;
+__device__ __forceinline__ int a_load_bytes(int valid) {
+  return valid > kFewRows ? kBM * kSlabBytes : (valid + 15) / 16 * 16 * kSlabBytes;
 }
 
 // WGRAD: a slab with `left` rows of its group left ends inside a k-step of 16.
 __device__ __forceinline__ bool slab_is_cut(int left, int slab) { return left < slab && (left & 15) != 0; }
 
-// One CTA a tile of 128 x W (W = 64, 128 or 256).
+// One CTA a tile of 128 x W (W <= 256; a multiple of 16, for an N-contiguous B of 64).
 template <Kind KIND, GMode MODE, Out OUT>
 __global__ void __launch_bounds__(kGroupedThreads, 1)
-    bw_tc_gemm_grouped_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
-                              const GroupedParams p) {
+    bw_tc_gemm_grouped_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmA16,
+                              const __grid_constant__ CUtensorMap tmB, const GroupedParams p) {
   constexpr int KE = KindTraits<KIND>::kElemsPerSlab;   // K elements a slab (WGRAD: rows)
   constexpr bool A_MN = MODE == GMode::WGRAD, B_MN = MODE != GMode::ROWS_NK;
   constexpr int kABytes = kBM * kSlabBytes;
@@ -262,7 +300,8 @@ __global__ void __launch_bounds__(kGroupedThreads, 1)
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   const int S = p.stages;
-  uint64_t* full = reinterpret_cast<uint64_t*>(smem + static_cast<size_t>(S) * p.stage_bytes);
+  uint8_t* staging = smem + static_cast<size_t>(S) * p.stage_bytes;
+  uint64_t* full = reinterpret_cast<uint64_t*>(staging + kEpiWarps * kEpiBufBytes);
   uint64_t* empty = full + kGroupedMaxStages;
   uint64_t* tailfull = empty + kGroupedMaxStages;  // WGRAD: a cut slab has landed, its rows behind the end still to clear
   uint64_t* fixed = tailfull + kGroupedMaxStages;  // ... and are cleared
@@ -292,9 +331,9 @@ __global__ void __launch_bounds__(kGroupedThreads, 1)
   // nothing is loaded (and the maps are empty) where nothing is summed
   if (warp == 0 && lane == 0 && (MODE == GMode::WGRAD ? p.rows : p.k) > 0) { tma_prefetch_desc(&tmA); tma_prefetch_desc(&tmB); }
   if (warp == 1) { tmem_alloc(tmem_slot, 512); tmem_relinquish(); }
-  if (warp == 2)
-    grouped_schedule(p.offsets, p.groups, p.rows, kBM, (p.n + p.W - 1) / p.W, bounds,
-                     MODE == GMode::WGRAD ? nullptr : tiles);
+  grouped_fetch(p.offsets, p.groups, p.rows, bounds);
+  __syncthreads();
+  if (warp == 2) grouped_scan(p.groups, kBM, (p.n + p.W - 1) / p.W, bounds, MODE == GMode::WGRAD ? nullptr : tiles);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -304,7 +343,7 @@ __global__ void __launch_bounds__(kGroupedThreads, 1)
 
   if (warp == 0) {
     // ---------------- TMA producer ----------------
-    if (lane == 0) {
+    if (elect_one()) {
       const uint64_t pol = l2_policy_evict_normal();
       int s = 0;
       uint32_t ph = 0;
@@ -315,7 +354,7 @@ __global__ void __launch_bounds__(kGroupedThreads, 1)
         const GTile o = walk.at(t);
         const int nk = (o.k + KE - 1) / KE;
         for (int kb = 0; kb < nk; ++kb) {
-          if (!mbar_wait(&empty[s], ph ^ 1, wc, 21)) { ok = false; break; }
+          if (!mbar_poll(&empty[s], ph ^ 1, wc, 21)) { ok = false; break; }
           uint8_t* sA = smem + static_cast<size_t>(s) * p.stage_bytes;
           uint8_t* sB = sA + kABytes;
           if constexpr (A_MN) {
@@ -336,8 +375,13 @@ __global__ void __launch_bounds__(kGroupedThreads, 1)
             for (int j = 0; j < p.W / 64; ++j)
               tma_load_2d(&tmB, bar, sB + j * kBoxBytes, o.col0 + 64 * j, o.kbase + kb * KE, pol);
           } else {
-            mbar_arrive_expect_tx(&full[s], p.stage_bytes);
-            tma_load_2d(&tmA, &full[s], sA, kb * KE, o.row0, pol);
+            mbar_arrive_expect_tx(&full[s], a_load_bytes(o.rows) + p.W * kSlabBytes);
+            if (o.rows > kFewRows) {
+              tma_load_2d(&tmA, &full[s], sA, kb * KE, o.row0, pol);
+            } else {
+              for (int r = 0; r < o.rows; r += 16)
+                tma_load_2d(&tmA16, &full[s], sA + r * kSlabBytes, kb * KE, o.row0 + r, pol);
+            }
             if constexpr (B_MN) {
               for (int j = 0; j < p.W / 64; ++j)
                 tma_load_3d(&tmB, &full[s], sB + j * kBoxBytes, o.col0 + 64 * j, kb * KE, o.g, pol);
@@ -358,7 +402,7 @@ __global__ void __launch_bounds__(kGroupedThreads, 1)
     }
   } else if (warp == 1) {
     // ---------------- MMA issuer ----------------
-    if (lane == 0) {
+    if (elect_one()) {
       const uint32_t idesc = idesc_dense(p.fmt, p.fmt, B_MN, kBM, p.W) | (A_MN ? 1u << 15 : 0u);
       int s = 0;
       uint32_t ph = 0, fixed_ph = 0;  // fixed_ph: one parity bit a stage
@@ -371,18 +415,18 @@ __global__ void __launch_bounds__(kGroupedThreads, 1)
         const int b = local & 1;
         const uint32_t aph = (local >> 1) & 1;
         ++local;
-        if (!mbar_wait(&accempty[b], aph ^ 1, wc, 22)) { ok = false; break; }
+        if (!mbar_poll(&accempty[b], aph ^ 1, wc, 22)) { ok = false; break; }
         tc_fence_after();
         const uint32_t d_tmem = tmem_base + b * 256;
         for (int kb = 0; kb < nk; ++kb) {
-          if (!mbar_wait(&full[s], ph, wc, 23)) { ok = false; break; }
+          if (!mbar_poll(&full[s], ph, wc, 23)) { ok = false; break; }
           int steps = 4;
           if constexpr (MODE == GMode::WGRAD) {
             const int left = o.k - kb * KE;
             if (left < KE) {
               steps = (left + 15) / 16;
               if (slab_is_cut(left, KE)) {
-                if (!mbar_wait(&fixed[s], (fixed_ph >> s) & 1u, wc, 24)) { ok = false; break; }
+                if (!mbar_poll(&fixed[s], (fixed_ph >> s) & 1u, wc, 24)) { ok = false; break; }
                 fixed_ph ^= 1u << s;
               }
             }
@@ -411,11 +455,12 @@ __global__ void __launch_bounds__(kGroupedThreads, 1)
   } else if (warp < 6) {
     // ---------------- epilogue ----------------
     const int q = warp & 3;
+    const uint32_t stage = smem_u32(staging) + q * kEpiBufBytes;
     int local = 0;
     for (int t = blockIdx.x; t < num_tiles; t += gridDim.x) {
       const GTile o = walk.at(t);
       if (o.k == 0) {
-        grouped_epilogue<MODE, OUT>(p, o, 0, q * 32, lane, [] {});
+        grouped_epilogue<MODE, OUT>(p, o, 0, q * 32, lane, stage, [] {});
         continue;
       }
       const int b = local & 1;
@@ -423,10 +468,11 @@ __global__ void __launch_bounds__(kGroupedThreads, 1)
       ++local;
       if (!mbar_wait_warp(&accfull[b], aph, wc, 25)) break;
       tc_fence_after();
-      grouped_epilogue<MODE, OUT>(p, o, tmem_base + (static_cast<uint32_t>(q * 32) << 16) + b * 256, q * 32, lane, [&] {
-        tc_fence_before();
-        mbar_arrive(&accempty[b]);
-      });
+      grouped_epilogue<MODE, OUT>(p, o, tmem_base + (static_cast<uint32_t>(q * 32) << 16) + b * 256, q * 32, lane, stage,
+                                  [&] {
+                                    tc_fence_before();
+                                    mbar_arrive(&accempty[b]);
+                                  });
     }
   } else if (MODE == GMode::WGRAD) {
     // ---------------- tail: clears rows between a group's end and the k-step's border ----------------
@@ -459,6 +505,300 @@ __global__ void __launch_bounds__(kGroupedThreads, 1)
     __syncwarp();
     tc_fence_after();
     tmem_dealloc(tmem_base, 512);
+  }
+}
+
+// ------------------------------------------------------------------------------------
+// CTA pairs: 256 x 256 tiles for groups with many rows. As in bw_gemm_pair.cuh, each CTA of a pair
+// loads its 128 rows of A and 128 columns of B, the leader's MMA thread multiplies both halves, and a
+// pipeline stage holds two swizzle atoms of K. Barriers: full[s], fixed[s] and accempty[b] count in
+// the leader; empty[s], accfull[b] and tailfull[s] exist in both CTAs.
+// ------------------------------------------------------------------------------------
+constexpr int kPairStages = 3, kPairSub = 2;  // stages, K atoms a stage
+constexpr int kPairAtom = 128 * kSlabBytes;
+constexpr int kPairStageBytes = 2 * kPairSub * kPairAtom;
+
+__device__ __forceinline__ void tma_load_3d_pair(const CUtensorMap* m, uint32_t bar_cluster, void* dst, int x, int y,
+                                                 int z, uint64_t policy) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes.L2::cache_hint"
+      " [%0], [%1, {%3, %4, %5}], [%2], %6;" ::"r"(smem_u32(dst)),
+      "l"(reinterpret_cast<uint64_t>(m)), "r"(bar_cluster), "r"(x), "r"(y), "r"(z), "l"(policy)
+      : "memory");
+}
+// Bounded wait that also acquires what the other CTA's threads wrote before they arrived.
+__device__ __forceinline__ bool mbar_wait_cluster(uint64_t* bar, uint32_t parity, const WaitCtl& w, int where) {
+  const uint32_t a = smem_u32(bar);
+  const uint64_t t0 = globaltimer_ns();
+  while (true) {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok)
+        : "r"(a), "r"(parity)
+        : "memory");
+    if (ok) return true;
+    if (*w.abort_flag) return false;
+    if (globaltimer_ns() - t0 > w.budget_ns) {
+      *w.abort_flag = 1;
+      atomicCAS(w.status, kDevOk, kDevTimeout * 256 + (where & 255));
+      return false;
+    }
+  }
+}
+
+template <Kind KIND, GMode MODE, Out OUT>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGroupedThreads, 1)
+    bw_tc_gemm_grouped_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmA16,
+                                   const __grid_constant__ CUtensorMap tmB, const GroupedParams p) {
+  constexpr int KA = KindTraits<KIND>::kElemsPerSlab;  // K elements an atom (WGRAD: rows)
+  constexpr int KE = KA * kPairSub;                    // ... a stage
+  constexpr bool A_MN = MODE == GMode::WGRAD, B_MN = MODE != GMode::ROWS_NK;
+  constexpr int kBoxBytes = 64 * kSlabBytes;
+  constexpr int S = kPairStages;
+  static_assert(KIND == Kind::F16 || (KIND == Kind::F8 && MODE == GMode::ROWS_NK), "8-bit operands are K-contiguous");
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint8_t* staging = smem + S * kPairStageBytes;
+  uint64_t* full = reinterpret_cast<uint64_t*>(staging + kEpiWarps * kEpiBufBytes);
+  uint64_t* empty = full + kGroupedMaxStages;
+  uint64_t* tailfull = empty + kGroupedMaxStages;
+  uint64_t* fixed = tailfull + kGroupedMaxStages;
+  uint64_t* accfull = fixed + kGroupedMaxStages;
+  uint64_t* accempty = accfull + 2;
+  uint64_t* teardown = accempty + 2;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(teardown + 1);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  int* bounds = reinterpret_cast<int*>(tmem_slot + 4);
+  int* tiles = bounds + p.groups + 1;
+
+  const int warp = threadIdx.x >> 5;
+  const int lane = threadIdx.x & 31;
+  const uint32_t rank = cluster_ctarank();
+  const bool leader = rank == 0;
+  const int cluster = blockIdx.x >> 1, nclusters = gridDim.x >> 1;
+  const int half = static_cast<int>(rank) * 128;  // this CTA's first row and column of a tile
+  const WaitCtl wc{abort_flag, p.status, p.budget_ns};
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < S; ++s) {
+      mbar_init(&full[s], 1);
+      mbar_init(&empty[s], 1);
+      mbar_init(&tailfull[s], 1);
+      mbar_init(&fixed[s], 2);
+    }
+    for (int b = 0; b < 2; ++b) { mbar_init(&accfull[b], 1); mbar_init(&accempty[b], 2 * kEpiWarps); }
+    mbar_init(teardown, 1);
+    *abort_flag = 0;
+    fence_mbar_init();
+  }
+  if (warp == 0 && lane == 0 && (MODE == GMode::WGRAD ? p.rows : p.k) > 0) { tma_prefetch_desc(&tmA); tma_prefetch_desc(&tmB); }
+  if (warp == 1) { tmem_alloc_pair(tmem_slot, 512); tmem_relinquish_pair(); }
+  grouped_fetch(p.offsets, p.groups, p.rows, bounds);
+  __syncthreads();
+  if (warp == 2) grouped_scan(p.groups, 256, (p.n + 255) / 256, bounds, MODE == GMode::WGRAD ? nullptr : tiles);
+  tc_fence_before();
+  __syncthreads();
+  cluster_sync();
+  tc_fence_after();
+  const uint32_t tmem_base = *tmem_slot;
+  GWalk<MODE, 256> walk(p, bounds, tiles);
+  const int num_tiles = walk.count();
+
+  if (warp == 0) {
+    // ---------------- TMA producer (both CTAs) ----------------
+    if (elect_one()) {
+      const uint64_t pol = l2_policy_evict_last();
+      const uint32_t full_leader = mapa_shared(smem_u32(full), 0);
+      int s = 0;
+      uint32_t ph = 0;
+      long long issued = 0;
+      uint32_t cut_last = 0, cut_ph = 0;
+      bool ok = true;
+      for (int t = cluster; t < num_tiles && ok; t += nclusters) {
+        const GTile o = walk.at(t);
+        const int nk = (o.k + KE - 1) / KE;
+        const int arow = o.row0 + half, bcol = o.col0 + half;
+        const int valid = min(128, o.rows - half);  // ROWS: this CTA's rows of the tile (may be <= 0)
+        const uint32_t a_bytes = a_load_bytes(min(128, o.rows)) + (o.rows > 128 ? a_load_bytes(o.rows - 128) : 0);
+        for (int kb = 0; kb < nk; ++kb) {
+          if (!mbar_poll(&empty[s], ph ^ 1, wc, 31)) { ok = false; break; }
+          uint8_t* sA = smem + s * kPairStageBytes;
+          uint8_t* sB = sA + kPairSub * kPairAtom;
+          uint32_t bar = full_leader + s * 8;
+          const int left = o.k - kb * KE;
+          const int atoms = left > KA ? 2 : 1;
+          if constexpr (A_MN) {
+            // a cut slab's two halves land on barriers of their own CTA's (see the single-CTA kernel)
+            if (slab_is_cut(left, KE)) {
+              if (leader) mbar_arrive(&full[s]);
+              bar = smem_u32(&tailfull[s]);
+              mbar_arrive_expect_tx(&tailfull[s], atoms * 2 * kPairAtom);
+              cut_last |= 1u << s;
+              cut_ph ^= 1u << s;
+            } else {
+              if (leader) mbar_arrive_expect_tx(&full[s], atoms * 4 * kPairAtom);
+              cut_last &= ~(1u << s);
+            }
+            for (int j = 0; j < atoms; ++j) {
+              const int y = o.kbase + kb * KE + j * KA;
+#pragma unroll
+              for (int i = 0; i < 2; ++i) {
+                tma_load_2d_pair(&tmA, bar, sA + j * kPairAtom + i * kBoxBytes, arow + 64 * i, y, pol);
+                tma_load_2d_pair(&tmB, bar, sB + j * kPairAtom + i * kBoxBytes, bcol + 64 * i, y, pol);
+              }
+            }
+          } else {
+            if (leader) mbar_arrive_expect_tx(&full[s], atoms * (a_bytes + 2 * kPairAtom));
+            for (int j = 0; j < atoms; ++j) {
+              const int x = kb * KE + j * KA;
+              if (valid > kFewRows) {
+                tma_load_2d_pair(&tmA, bar, sA + j * kPairAtom, x, arow, pol);
+              } else {
+                for (int r = 0; r < valid; r += 16)
+                  tma_load_2d_pair(&tmA16, bar, sA + j * kPairAtom + r * kSlabBytes, x, arow + r, pol);
+              }
+              if constexpr (B_MN) {
+                tma_load_3d_pair(&tmB, bar, sB + j * kPairAtom, bcol, x, o.g, pol);
+                tma_load_3d_pair(&tmB, bar, sB + j * kPairAtom + kBoxBytes, bcol + 64, x, o.g, pol);
+              } else {
+                tma_load_3d_pair(&tmB, bar, sB + j * kPairAtom, x, bcol, o.g, pol);
+              }
+            }
+          }
+          ++issued;
+          if (++s == S) { s = 0; ph ^= 1; }
+        }
+      }
+      if (!ok)  // a timeout: loads in flight land before the CTAs end (the leader counts both CTAs' on full)
+        for (long long i = issued > S ? issued - S : 0; i < issued; ++i) {
+          const int st = static_cast<int>(i % S);
+          if ((cut_last >> st) & 1u) mbar_drain(&tailfull[st], ((cut_ph >> st) & 1u) ^ 1u, p.budget_ns);
+          else if (leader) mbar_drain(&full[st], static_cast<uint32_t>(i / S) & 1u, p.budget_ns);
+        }
+    }
+  } else if (warp == 1) {
+    // ---------------- MMA issuer (leader CTA only) ----------------
+    if (leader && elect_one()) {
+      const uint32_t idesc = idesc_dense(p.fmt, p.fmt, B_MN, 256, 256) | (A_MN ? 1u << 15 : 0u);
+      const uint32_t empty_own = smem_u32(empty), empty_peer = mapa_shared(smem_u32(empty), 1);
+      const uint32_t accfull_own = smem_u32(accfull), accfull_peer = mapa_shared(smem_u32(accfull), 1);
+      int s = 0;
+      uint32_t ph = 0, fixed_ph = 0;
+      int local = 0;
+      bool ok = true;
+      for (int t = cluster; t < num_tiles && ok; t += nclusters) {
+        const GTile o = walk.at(t);
+        const int nk = (o.k + KE - 1) / KE;
+        if (nk == 0) continue;
+        const int b = local & 1;
+        const uint32_t aph = (local >> 1) & 1;
+        ++local;
+        if (!mbar_poll(&accempty[b], aph ^ 1, wc, 32)) { ok = false; break; }
+        tc_fence_after();
+        const uint32_t d_tmem = tmem_base + b * 256;
+        for (int kb = 0; kb < nk; ++kb) {
+          if (!mbar_poll(&full[s], ph, wc, 33)) { ok = false; break; }
+          const int left = o.k - kb * KE;
+          // WGRAD: k-steps with rows of the group; else whole atoms (zeros behind K)
+          int steps = 4 * kPairSub;
+          if (left < KE) steps = MODE == GMode::WGRAD ? (left + 15) / 16 : (left > KA ? 8 : 4);
+          if (MODE == GMode::WGRAD && slab_is_cut(left, KE)) {
+            if (!mbar_wait_cluster(&fixed[s], (fixed_ph >> s) & 1u, wc, 34)) { ok = false; break; }
+            fixed_ph ^= 1u << s;
+          }
+          tc_fence_after();
+          const uint32_t aaddr = smem_u32(smem + s * kPairStageBytes);
+          const uint32_t baddr = aaddr + kPairSub * kPairAtom;
+          auto step = [&](int kk) {
+            const int j = kk >> 2, k = kk & 3;
+            const uint32_t acc = (kb > 0 || kk > 0) ? 1u : 0u;
+            uint64_t adesc, bdesc;
+            if constexpr (A_MN) adesc = sdesc_sw128(aaddr + j * kPairAtom + k * 16 * kSlabBytes, kBoxBytes, 1024);
+            else adesc = sdesc_sw128(aaddr + j * kPairAtom + k * 32, 16, 1024);
+            if constexpr (B_MN) bdesc = sdesc_sw128(baddr + j * kPairAtom + k * 16 * kSlabBytes, kBoxBytes, 1024);
+            else bdesc = sdesc_sw128(baddr + j * kPairAtom + k * 32, 16, 1024);
+            if constexpr (KIND == Kind::F16) umma_f16_pair(d_tmem, adesc, bdesc, idesc, acc);
+            else umma_f8f6f4_pair(d_tmem, adesc, bdesc, idesc, acc);
+          };
+          if (steps == 4 * kPairSub) {
+#pragma unroll
+            for (int kk = 0; kk < 4 * kPairSub; ++kk) step(kk);
+          } else {
+            for (int kk = 0; kk < steps; ++kk) step(kk);
+          }
+          umma_commit_pair(empty_own + s * 8);
+          umma_commit_pair(empty_peer + s * 8);
+          if (++s == S) { s = 0; ph ^= 1; }
+        }
+        if (ok) {
+          umma_commit_pair(accfull_own + b * 8);
+          umma_commit_pair(accfull_peer + b * 8);
+        }
+      }
+      umma_commit_pair(smem_u32(teardown));
+      mbar_drain(teardown, 0, p.budget_ns);
+    }
+  } else if (warp < 6) {
+    // ---------------- epilogue (both CTAs) ----------------
+    const int q = warp & 3;
+    const uint32_t accempty_leader = mapa_shared(smem_u32(accempty), 0);
+    const uint32_t stage = smem_u32(staging) + q * kEpiBufBytes;
+    int local = 0;
+    for (int t = cluster; t < num_tiles; t += nclusters) {
+      const GTile o = walk.at(t);
+      if (o.k == 0) {
+        grouped_epilogue<MODE, OUT>(p, o, 0, half + q * 32, lane, stage, [] {});
+        continue;
+      }
+      const int b = local & 1;
+      const uint32_t aph = (local >> 1) & 1;
+      ++local;
+      if (!mbar_wait_warp(&accfull[b], aph, wc, 35)) break;
+      tc_fence_after();
+      grouped_epilogue<MODE, OUT>(p, o, tmem_base + (static_cast<uint32_t>(q * 32) << 16) + b * 256, half + q * 32, lane,
+                                  stage, [&] {
+                                    tc_fence_before();
+                                    __syncwarp();
+                                    if (lane == 0) mbar_arrive_remote_cta(accempty_leader + b * 8);
+                                  });
+    }
+  } else if (MODE == GMode::WGRAD) {
+    // ---------------- tail (both CTAs, each its own halves) ----------------
+    const uint32_t fixed_leader = mapa_shared(smem_u32(fixed), 0);
+    long long issue = 0;
+    uint32_t cut_ph = 0;
+    for (int t = cluster; t < num_tiles; t += nclusters) {
+      const GTile o = walk.at(t);
+      const int nk = (o.k + KE - 1) / KE;
+      const int left = o.k - (nk - 1) * KE;
+      issue += nk;
+      if (nk == 0 || !slab_is_cut(left, KE)) continue;
+      const int s = static_cast<int>((issue - 1) % S);
+      if (!mbar_wait_warp(&tailfull[s], (cut_ph >> s) & 1u, wc, 36)) break;
+      cut_ph ^= 1u << s;
+      const int j = left / KA, at = left - j * KA;  // atom and row of the first row behind the end
+      const uint32_t base = smem_u32(smem + s * kPairStageBytes) + j * kPairAtom;
+      const int nz = ((left + 15) & ~15) - left;
+      for (int i = lane; i < 4 * nz * 8; i += 32) {  // boxes: A, A + 64 columns, B, B + 64 columns
+        const int box = i / (nz * 8), rest = i - box * nz * 8;
+        st_shared_v4(base + (box >> 1) * kPairSub * kPairAtom + (box & 1) * kBoxBytes + (at + rest / 8) * kSlabBytes +
+                         (rest & 7) * 16, 0, 0, 0, 0);
+      }
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) mbar_arrive_cluster(fixed_leader + s * 8);
+    }
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  cluster_sync();
+  if (warp == 1) {
+    __syncwarp();
+    tc_fence_after();
+    tmem_dealloc_pair(tmem_base, 512);
   }
 }
 

@@ -6,6 +6,7 @@
 #include <cuda_runtime.h>
 
 #include <cstdint>
+#include <cstdlib>
 #include <string>
 
 #include "../../include/bwgemm.h"
@@ -56,6 +57,34 @@ int make_tmap_3d(CUtensorMap* map, CUtensorMapDataType dtype, const void* base, 
 
 // [world][M][N/world] -> row-major M x N for 4-byte (FP32) or 2-byte (BF16) elements.
 int unshard_elems(const void* src, void* dst, int M, int N, int world, int elem_bytes, cudaStream_t stream);
+
+inline int env_int(const char* name, int dflt) {
+  const char* s = getenv(name);
+  return s && *s ? atoi(s) : dflt;
+}
+
+// Co-resident CTA pairs of a persistent `__cluster_dims__(2,1,1)` kernel (clusters must fit
+// inside one GPC, so this can be below sms / 2); falls back to sms / 2 if the query fails.
+template <typename Kernel>
+int pair_clusters_resident(Kernel kern, int threads, int smem_bytes, const DeviceState& d) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(2 * (d.sms / 2), 1, 1);
+  cfg.blockDim = dim3(threads, 1, 1);
+  cfg.dynamicSmemBytes = smem_bytes;
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeClusterDimension;
+  attr.val.clusterDim.x = 2;
+  attr.val.clusterDim.y = 1;
+  attr.val.clusterDim.z = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  int n = 0;
+  if (cudaOccupancyMaxActiveClusters(&n, kern, &cfg) != cudaSuccess || n <= 0) {
+    cudaGetLastError();
+    n = d.sms / 2;
+  }
+  return n;
+}
 
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 

@@ -110,6 +110,32 @@ def test_rows(cuda_dev, offsets, rows, n, k, kind, layout, out):
     _check_rows(cuda_dev, kind, layout, offsets, rows, n, k, out, seed=rows + n)
 
 
+VARIANTS = [{"BW_GROUPED_PAIR": "1"}, {"BW_GROUPED_PAIR": "0", "BW_GROUPED_W": "64"},
+            {"BW_GROUPED_PAIR": "0", "BW_GROUPED_W": "128"}, {"BW_GROUPED_PAIR": "0", "BW_GROUPED_W": "256"},
+            {"BW_GROUPED_PAIR": "0", "BW_GROUPED_W": "176"}]
+
+
+@pytest.mark.parametrize("env", VARIANTS, ids=["pair", "w64", "w128", "w256", "w176"])
+@pytest.mark.parametrize("case", [1, 3, 4, 6])
+def test_every_tile_shape(cuda_dev, monkeypatch, env, case):
+    """The kernels and tile widths that the sizes would not choose by themselves, forward and gradients."""
+    import torch
+
+    for k, v in env.items():
+        monkeypatch.setenv(k, v)
+    offsets, rows, n, k = ROWS[case]
+    for kind, layout in (("float16", "kn"), ("bfloat16", "nk"), ("fp8", "nk")):
+        for out in (F32, BF16):
+            _check_rows(cuda_dev, kind, layout, offsets, rows, n, k, out, seed=case)
+    g = torch.Generator(device=cuda_dev).manual_seed(case)
+    x = torch.randn(rows, k, device=cuda_dev, generator=g).bfloat16()
+    y = torch.randn(rows, n, device=cuda_dev, generator=g).bfloat16()
+    off = torch.tensor(offsets, dtype=torch.int32, device=cuda_dev)
+    for out in (F32, BF16):
+        _check_wgrad(x, y, offsets, bwgemm.gemm_grouped_wgrad(x, y, off, out_dtype=out), out)
+    assert bwgemm.device_status() == 0
+
+
 @pytest.mark.parametrize("n", [1, 3, 17, 65, 127, 250, 257, 511])
 @pytest.mark.parametrize("out", [F32, BF16])
 def test_odd_columns(cuda_dev, n, out):
