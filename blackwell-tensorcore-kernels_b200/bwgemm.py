@@ -413,8 +413,10 @@ def rmsnorm(x, weight, residual=None, eps: float = 1e-6, y=None, h=None, rstd=No
     with _scope(x, stream):
         h, ldh, hout, rstd = _norm_outputs(x, shape, dtype, dev, residual, h, rstd)
         if y is None:
-            y = torch.empty_strided(shape, (shape[1], 1), dtype=dtype, device=x.device)
-        ldy = _rows("y", y, shape, dtype, dev)
+            ldy = shape[1]
+            y = torch.empty_strided(shape, (ldy, 1), dtype=dtype, device=x.device)
+        else:
+            ldy = _rows("y", y, shape, dtype, dev)
         _check(lib().bw_rmsnorm(x.data_ptr(), ldx, _ptr(residual), ldr, weight.data_ptr(), code, wcode, eps,
                                 y.data_ptr(), ldy, _ptr(hout), ldh, rstd.data_ptr(), shape[0], shape[1],
                                 _current_stream(dev)))
@@ -430,8 +432,10 @@ def rmsnorm_fp8(x, weight, residual=None, eps: float = 1e-6, q=None, row_scale=N
     with _scope(x, stream):
         h, ldh, hout, rstd = _norm_outputs(x, shape, dtype, dev, residual, h, rstd)
         if q is None:
-            q = torch.empty_strided(shape, (shape[1], 1), dtype=torch.uint8, device=x.device)
-        ldq = _rows("q", q, shape, torch.uint8, dev)
+            ldq = shape[1]
+            q = torch.empty_strided(shape, (ldq, 1), dtype=torch.uint8, device=x.device)
+        else:
+            ldq = _rows("q", q, shape, torch.uint8, dev)
         if row_scale is None:
             row_scale = torch.empty_strided((shape[0],), (1,), dtype=torch.float32, device=x.device)
         else:
@@ -454,8 +458,10 @@ def rmsnorm_backward(dy, h, weight, rstd, dresidual=None, dx=None, dweight=None,
     _flat("rstd", rstd, shape[:1], torch.float32, dev)
     with _scope(h, stream):
         if dx is None:
-            dx = torch.empty_strided(shape, (shape[1], 1), dtype=dtype, device=h.device)
-        lddx = _rows("dx", dx, shape, dtype, dev)
+            lddx = shape[1]
+            dx = torch.empty_strided(shape, (lddx, 1), dtype=dtype, device=h.device)
+        else:
+            lddx = _rows("dx", dx, shape, dtype, dev)
         if dweight is None:
             dweight = torch.empty_strided((shape[1],), (1,), dtype=torch.float32, device=h.device)
         else:
@@ -518,8 +524,10 @@ def gemm_grouped(A, B, offsets, C=None, b_transposed: bool = False, row_scale=No
     otype = _out_type(out_dtype)
     with _scope(A, stream):
         if C is None:
+            ldc = N
             C = torch.empty_strided((rows, N), (N, 1), dtype=otype, device=A.device)
-        ldc = _rows("C", C, (rows, N), otype, dev)
+        else:
+            ldc = _rows("C", C, (rows, N), otype, dev)
         _check(lib().bw_gemm_grouped(code, A.data_ptr(), lda, B.data_ptr(), int(b_transposed), offsets.data_ptr(),
                                      groups, _ptr(row_scale), _ptr(group_scale), C.data_ptr(), ldc, out_dtype, rows,
                                      N, K, _current_stream(dev)))
@@ -543,7 +551,8 @@ def gemm_grouped_wgrad(X, Y, offsets, D=None, out_dtype=OUT_F32, stream=None):
     with _scope(X, stream):
         if D is None:
             D = torch.empty_strided((groups, M, N), (M * N, N, 1), dtype=otype, device=X.device)
-        _flat("D", D, (groups, M, N), otype, dev)
+        else:
+            _flat("D", D, (groups, M, N), otype, dev)
         _check(lib().bw_gemm_grouped_wgrad(code, X.data_ptr(), ldx, Y.data_ptr(), ldy, offsets.data_ptr(), groups,
                                            D.data_ptr(), out_dtype, rows, M, N, _current_stream(dev)))
     return D

@@ -9,15 +9,19 @@
 //   dx_j = rstd (dy_j w_j - n_j mean_i(dy_i w_i n_i)) + dresidual_j,      dw_j = sum over rows of dy_j n_j
 //
 // Both are bound by memory: every input is read once and every output written once. A row stays
-// in registers (packed in its own type: h is rounded to it anyway) between its reduction and its
-// output. max |y| needs no second reduction: y_j = (h_j w_j) rstd and rounding is monotonic, so
-// max |y| = max |h w| * rstd exactly, and both sums travel through one reduction. Statistics and
-// sums are FP32.
+// in registers (packed in its own type: h is rounded to it anyway, and h w in FP32) between its
+// reduction and its output. max |y| needs no second reduction: y_j = (h_j w_j) rstd and rounding is
+// monotonic, so max |y| = max |h w| * rstd exactly, and both sums travel through one reduction.
+// Statistics and sums are FP32. Measured, 16384 x 8192 BF16 with residual: to E4M3 140 us (6.7 TB/s of
+// the 7 bytes an element), gradient 178 us (6.0 TB/s of 8 bytes); 131072 x 128 BF16 to BF16 11.0 us
+// (6.2 TB/s); 8192 x 4095 to E4M3, rows at every alignment, 50 us; one row of 8192 3 us.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_fp8.h>
 
+#include <atomic>
 #include <cmath>
+#include <type_traits>
 
 #include "bw_runtime.cuh"
 
@@ -31,79 +35,185 @@ __device__ __forceinline__ float to_f32(float v) { return v; }
 __device__ __forceinline__ float to_f32(__half v) { return __half2float(v); }
 __device__ __forceinline__ float to_f32(__nv_bfloat16 v) { return __bfloat162float(v); }
 template <typename T>
-__device__ __forceinline__ T from_f32(float v);
-template <>
-__device__ __forceinline__ float from_f32<float>(float v) { return v; }
-template <>
-__device__ __forceinline__ __half from_f32<__half>(float v) { return __float2half_rn(v); }
-template <>
-__device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
+__device__ __forceinline__ T from_f32(float v) {
+  if constexpr (sizeof(T) == 4) return v;
+  else if constexpr (std::is_same_v<T, __half>) return __float2half_rn(v);
+  else return __float2bfloat16_rn(v);
+}
 
-// VE consecutive elements, moved as one access of VE * sizeof(T) bytes.
-template <typename T, int VE>
-struct alignas(sizeof(T) * VE) Pack {
-  T v[VE];
-};
+// VE consecutive elements in whole registers, moved as one access of VE * sizeof(T) bytes (an array
+// of 16-bit elements would take a register each).
 template <int BYTES>
-struct RawOf;
-template <> struct RawOf<1> { using type = uint8_t; };
-template <> struct RawOf<2> { using type = uint16_t; };
-template <> struct RawOf<4> { using type = uint32_t; };
-template <> struct RawOf<8> { using type = uint2; };
-template <> struct RawOf<16> { using type = uint4; };
+struct Words {
+  static_assert(BYTES == 4 || BYTES == 8 || BYTES == 16 || BYTES == 32, "a power of two of words");
+  uint32_t u[BYTES / 4];
+};
+template <>
+struct Words<2> {
+  uint32_t u[1];
+};
+template <>
+struct Words<1> {
+  uint32_t u[1];
+};
 template <typename T, int VE>
-__device__ __forceinline__ Pack<T, VE> load_pack(const T* p) {
-  using Raw = typename RawOf<sizeof(T) * VE>::type;
-  const Raw raw = *reinterpret_cast<const Raw*>(p);
-  Pack<T, VE> v;
-  __builtin_memcpy(&v, &raw, sizeof(v));
+using Vec = Words<sizeof(T) * VE>;
+
+template <int BYTES>
+__device__ __forceinline__ Words<BYTES> load_words(const void* p) {
+  Words<BYTES> v;
+  if constexpr (BYTES == 1) {
+    v.u[0] = *static_cast<const uint8_t*>(p);
+  } else if constexpr (BYTES == 2) {
+    v.u[0] = *static_cast<const uint16_t*>(p);
+  } else if constexpr (BYTES == 4) {
+    v.u[0] = *static_cast<const uint32_t*>(p);
+  } else if constexpr (BYTES == 8) {
+    const uint2 x = *static_cast<const uint2*>(p);
+    v.u[0] = x.x;
+    v.u[1] = x.y;
+  } else {
+#pragma unroll
+    for (int i = 0; i < BYTES / 16; ++i) {
+      const uint4 x = static_cast<const uint4*>(p)[i];
+      v.u[4 * i] = x.x;
+      v.u[4 * i + 1] = x.y;
+      v.u[4 * i + 2] = x.z;
+      v.u[4 * i + 3] = x.w;
+    }
+  }
   return v;
 }
-template <typename T, int VE>
-__device__ __forceinline__ void store_pack(T* p, const Pack<T, VE>& v) {
-  using Raw = typename RawOf<sizeof(T) * VE>::type;
-  Raw raw;
-  __builtin_memcpy(&raw, &v, sizeof(v));
-  *reinterpret_cast<Raw*>(p) = raw;
+template <int BYTES>
+__device__ __forceinline__ void store_words(void* p, const Words<BYTES>& v) {
+  if constexpr (BYTES == 1) *static_cast<uint8_t*>(p) = static_cast<uint8_t>(v.u[0]);
+  else if constexpr (BYTES == 2) *static_cast<uint16_t*>(p) = static_cast<uint16_t>(v.u[0]);
+  else if constexpr (BYTES == 4) *static_cast<uint32_t*>(p) = v.u[0];
+  else if constexpr (BYTES == 8) *static_cast<uint2*>(p) = make_uint2(v.u[0], v.u[1]);
+  else *static_cast<uint4*>(p) = make_uint4(v.u[0], v.u[1], v.u[2], v.u[3]);
 }
-
-// VE weights from column c, of x's type or FP32.
-template <typename T, int VE>
-__device__ __forceinline__ void load_weight(const void* w, int w_f32, long long c, float (&out)[VE]) {
-  if (w_f32) {
-    constexpr int F = VE < 4 ? VE : 4;
+template <int BYTES>
+__device__ __forceinline__ Words<BYTES> zero_words() {
+  Words<BYTES> v;
 #pragma unroll
-    for (int i = 0; i < VE / F; ++i) {
-      const Pack<float, F> f = load_pack<float, F>(static_cast<const float*>(w) + c + F * i);
-#pragma unroll
-      for (int j = 0; j < F; ++j) out[F * i + j] = f.v[j];
-    }
+  for (int i = 0; i < (BYTES + 3) / 4; ++i) v.u[i] = 0;
+  return v;
+}
+// Element j of a vector as FP32, and two FP32 values as elements 2 i, 2 i + 1.
+template <typename T, int BYTES>
+__device__ __forceinline__ float elem(const Words<BYTES>& v, int j) {
+  if constexpr (sizeof(T) == 4) {
+    return __uint_as_float(v.u[j]);
+  } else if constexpr (std::is_same_v<T, __half>) {
+    return __half2float(__ushort_as_half(static_cast<unsigned short>(v.u[j / 2] >> (16 * (j & 1)))));
   } else {
-    const Pack<T, VE> f = load_pack<T, VE>(static_cast<const T*>(w) + c);
-#pragma unroll
-    for (int j = 0; j < VE; ++j) out[j] = to_f32(f.v[j]);
+    return __uint_as_float(j & 1 ? v.u[j / 2] & 0xffff0000u : v.u[j / 2] << 16);
   }
 }
+template <typename T>
+__device__ __forceinline__ uint32_t two_elems(float a, float b) {
+  if constexpr (std::is_same_v<T, __half>) {
+    const __half2 h = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  } else {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  }
+}
+template <typename T, int VE>
+__device__ __forceinline__ Vec<T, VE> from_floats(const float (&f)[VE]) {
+  Vec<T, VE> v;
+  if constexpr (sizeof(T) == 4) {
+#pragma unroll
+    for (int j = 0; j < VE; ++j) v.u[j] = __float_as_uint(f[j]);
+  } else if constexpr (VE == 1) {
+    v.u[0] = two_elems<T>(f[0], 0.f);
+  } else {
+#pragma unroll
+    for (int j = 0; j < VE; j += 2) v.u[j / 2] = two_elems<T>(f[j], f[j + 1]);
+  }
+  return v;
+}
 
-// Reduction over the `tpr` threads of a row: part of a warp (tpr <= 32), or the whole block.
-// `slot` alternates between two halves of `sm`, so one barrier a call is enough.
+// What a thread holds of a row: vectors i at columns col(i) .. col(i) + VE - 1, all of them whole. Where the
+// row starts behind a vector's boundary (SHIFT), the elements in front of the first boundary and behind
+// the last are left, at most VE - 1 each: 16 threads of the row hold one of them each, at column
+// `single`. (Edge vectors of which parts count cost the two threads that had them, and with them
+// the whole row, three times as long as everything else.)
+template <int VE, bool SHIFT>
+struct Columns {
+  int tpr, t, front, vecs, single;
+  __device__ __forceinline__ Columns(int tpr_, int t_, int phase, int cols) : tpr(tpr_), t(t_), front(0), single(-1) {
+    if constexpr (SHIFT) front = min((VE - phase) & (VE - 1), cols);
+    vecs = (cols - front) / VE;
+    if constexpr (SHIFT) {
+      const int behind = front + vecs * VE + t - 8;
+      if (t < front) single = t;
+      else if (t >= 8 && t < 16 && behind < cols) single = behind;
+    }
+  }
+  __device__ __forceinline__ int col(int i) const { return front + (i * tpr + t) * VE; }
+  __device__ __forceinline__ bool has(int i) const { return i * tpr + t < vecs; }
+};
+template <typename T, int VE, int NV, bool SHIFT>
+struct Part {
+  Vec<T, VE> v[NV];
+  float one;  // the single element
+};
+
+template <typename T, int VE, int NV, bool SHIFT>
+__device__ __forceinline__ void load_row(const T* row, const Columns<VE, SHIFT>& c, Part<T, VE, NV, SHIFT>& o) {
+#pragma unroll
+  for (int i = 0; i < NV; ++i)
+    o.v[i] = c.has(i) ? load_words<sizeof(T) * VE>(row + c.col(i)) : zero_words<sizeof(T) * VE>();
+  if constexpr (SHIFT) o.one = c.single >= 0 ? to_f32(row[c.single]) : 0.f;
+}
+template <typename T, int VE, int NV, bool SHIFT>
+__device__ __forceinline__ void store_row(T* row, const Columns<VE, SHIFT>& c, const Part<T, VE, NV, SHIFT>& o) {
+#pragma unroll
+  for (int i = 0; i < NV; ++i)
+    if (c.has(i)) store_words<sizeof(T) * VE>(row + c.col(i), o.v[i]);
+  if constexpr (SHIFT)
+    if (c.single >= 0) row[c.single] = from_f32<T>(o.one);
+}
+// The weights have an alignment of their own: SHIFT reads them one by one (once for all rows of a
+// thread, unless they do not fit its registers).
+template <typename WT, int VE, bool SHIFT>
+__device__ __forceinline__ Vec<WT, VE> load_weight(const void* w, const Columns<VE, SHIFT>& c, int i) {
+  Vec<WT, VE> v = zero_words<sizeof(WT) * VE>();
+  if (!c.has(i)) return v;
+  const WT* p = static_cast<const WT*>(w) + c.col(i);
+  if constexpr (SHIFT) {
+#pragma unroll
+    for (int j = 0; j < VE; ++j)
+      v.u[j * sizeof(WT) / 4] |= load_words<sizeof(WT)>(p + j).u[0] << (8 * (j * sizeof(WT) % 4));
+  } else {
+    v = load_words<sizeof(WT) * VE>(p);
+  }
+  return v;
+}
+
+// Reduction over the `tpr` threads of a row: part of a warp (a power of two up to 32), or the whole
+// block (up to 32 warps). All threads get the result. A caller in a loop alternates between two `sm`,
+// so one barrier a call is enough.
 struct SumMax {
   float sum, max;
 };
-__device__ __forceinline__ SumMax reduce_row(SumMax v, int tpr, SumMax* sm) {
-  for (int o = (tpr < 32 ? tpr : 32) / 2; o > 0; o >>= 1) {
+__device__ __forceinline__ SumMax reduce_lanes(SumMax v, int width) {
+  for (int o = width / 2; o > 0; o >>= 1) {
     v.sum += __shfl_xor_sync(0xffffffffu, v.sum, o);
     v.max = fmaxf(v.max, __shfl_xor_sync(0xffffffffu, v.max, o));
   }
+  return v;
+}
+__device__ __forceinline__ SumMax reduce_row(SumMax v, int tpr, SumMax* sm) {
+  v = reduce_lanes(v, tpr < 32 ? tpr : 32);
   if (tpr > 32) {
-    const int warps = tpr >> 5;
-    if ((threadIdx.x & 31) == 0) sm[threadIdx.x >> 5] = v;
+    const int warps = tpr >> 5, lane = threadIdx.x & 31;
+    if (lane == 0) sm[threadIdx.x >> 5] = v;
     __syncthreads();
-    v = sm[(threadIdx.x & 31) % warps];  // warps is a power of two: every lane ends with the whole
-    for (int o = warps / 2; o > 0; o >>= 1) {
-      v.sum += __shfl_xor_sync(0xffffffffu, v.sum, o);
-      v.max = fmaxf(v.max, __shfl_xor_sync(0xffffffffu, v.max, o));
-    }
+    v = lane < warps ? sm[lane] : SumMax{0.f, 0.f};  // maxima are of magnitudes
+    v = reduce_lanes(v, 32);
   }
   return v;
 }
@@ -121,6 +231,7 @@ struct NormParams {
   long long rows;
   int cols;
   float eps;
+  int phase;           // elements between a vector's boundary and the first row (SHIFT)
 };
 
 // Scale of an E4M3 row by its maximum, and the factor that quantises it. A maximum so small that
@@ -138,123 +249,157 @@ __device__ __forceinline__ void e4m3_row_scale(float amax, float& mul, float& s)
 }
 
 template <int VE>
-__device__ __forceinline__ Pack<uint8_t, VE> encode_e4m3(const float (&y)[VE], float mul) {
-  Pack<uint8_t, VE> q;
+__device__ __forceinline__ Words<VE> encode_e4m3(const float (&y)[VE], float mul) {
+  Words<VE> q = zero_words<VE>();
   if constexpr (VE % 2 == 0) {
 #pragma unroll
     for (int j = 0; j < VE; j += 2) {
       const __nv_fp8x2_storage_t two =
           __nv_cvt_float2_to_fp8x2(make_float2(y[j] * mul, y[j + 1] * mul), __NV_SATFINITE, __NV_E4M3);
-      q.v[j] = static_cast<uint8_t>(two & 0xff);
-      q.v[j + 1] = static_cast<uint8_t>(two >> 8);
+      q.u[j / 4] |= static_cast<uint32_t>(two) << (8 * (j % 4));
     }
   } else {
-#pragma unroll
-    for (int j = 0; j < VE; ++j) q.v[j] = static_cast<uint8_t>(__nv_cvt_float_to_fp8(y[j] * mul, __NV_SATFINITE, __NV_E4M3));
+    q.u[0] = __nv_cvt_float_to_fp8(y[0] * mul, __NV_SATFINITE, __NV_E4M3);
   }
   return q;
 }
 
-template <typename T, bool Q8, int VE>
-__device__ __forceinline__ void write_out(const NormParams& p, long long row, long long c, const Pack<T, VE>& h,
-                                          float rstd, float mul) {
-  float w[VE], y[VE];
-  load_weight<T, VE>(p.w, p.w_f32, c, w);
-#pragma unroll
-  for (int j = 0; j < VE; ++j) y[j] = to_f32(h.v[j]) * w[j] * rstd;
-  if constexpr (Q8) {
-    store_pack<uint8_t, VE>(static_cast<uint8_t*>(p.y) + row * p.ldy + c, encode_e4m3<VE>(y, mul));
-  } else {
-    Pack<T, VE> o;
-#pragma unroll
-    for (int j = 0; j < VE; ++j) o.v[j] = from_f32<T>(y[j]);
-    store_pack<T, VE>(static_cast<T*>(p.y) + row * p.ldy + c, o);
-  }
-}
-
-// h of one vector: x, or x + residual rounded to T and stored.
 template <typename T, int VE>
-__device__ __forceinline__ void add_residual(Pack<T, VE>& h, const Pack<T, VE>& r) {
+__device__ __forceinline__ void add_residual(Vec<T, VE>& h, const Vec<T, VE>& r) {
+  float f[VE];
 #pragma unroll
-  for (int j = 0; j < VE; ++j) h.v[j] = from_f32<T>(to_f32(h.v[j]) + to_f32(r.v[j]));
+  for (int j = 0; j < VE; ++j) f[j] = elem<T>(h, j) + elem<T>(r, j);
+  h = from_floats<T, VE>(f);
 }
 
-template <typename T, bool Q8, int VE>
-__device__ __forceinline__ void accumulate(const NormParams& p, long long c, const Pack<T, VE>& h, SumMax& a) {
-  float w[VE];
-  if constexpr (Q8) load_weight<T, VE>(p.w, p.w_f32, c, w);
+// p = h w, and its share of the row's sums.
+template <bool Q8, typename T, typename WT, int VE>
+__device__ __forceinline__ void accumulate(const Vec<T, VE>& h, const Vec<WT, VE>& w, float (&p)[VE], SumMax& a) {
 #pragma unroll
   for (int j = 0; j < VE; ++j) {
-    const float v = to_f32(h.v[j]);
+    const float v = elem<T>(h, j);
+    p[j] = v * elem<WT>(w, j);
     a.sum = fmaf(v, v, a.sum);
-    if constexpr (Q8) a.max = fmaxf(a.max, fabsf(v * w[j]));
+    if constexpr (Q8) a.max = fmaxf(a.max, fabsf(p[j]));
   }
 }
 
+// Writes a row's rstd (and scale). Returns the factor from h w to y, or to the code's value; where that
+// overflows (a row of tiny values), `pre` is a first factor of its own, else 1.
 template <bool Q8>
-__device__ __forceinline__ float finish_row(const NormParams& p, long long row, const SumMax& a, bool first,
-                                            float& mul) {
+__device__ __forceinline__ float finish_row(const NormParams& p, long long row, const SumMax& a, bool first, float& pre) {
   const float rstd = 1.f / sqrtf(a.sum / static_cast<float>(p.cols) + p.eps);
-  mul = 1.f;
-  float s = 1.f;
+  float mul = 1.f, s = 1.f;
   if constexpr (Q8) e4m3_row_scale(a.max * rstd, mul, s);
   if (first) {
     if (p.rstd) p.rstd[row] = rstd;
     if constexpr (Q8) p.row_scale[row] = s;
   }
-  return rstd;
+  const float f = rstd * mul;
+  pre = 1.f;
+  if (!Q8 || f < INFINITY) return f;
+  pre = rstd;
+  return mul;
 }
 
-// tpr threads a row (a power of two), NV vectors of VE elements a thread: the row is read once
-// and kept. blockDim.x = tpr for tpr > 32, else a block holds blockDim.x / tpr rows.
-template <typename T, bool Q8, int VE, int NV>
-__global__ void __launch_bounds__(1024) k_rmsnorm(const NormParams p, int tpr) {
-  __shared__ SumMax sm[32];
-  const int t = threadIdx.x & (tpr - 1);
-  const long long row = static_cast<long long>(blockIdx.x) * (blockDim.x / tpr) + threadIdx.x / tpr;
-  const bool live = row < p.rows;
-  const T* x = static_cast<const T*>(p.x) + row * p.ldx;
-  const T* r = p.res ? static_cast<const T*>(p.res) + row * p.ldr : nullptr;
-  Pack<T, VE> h[NV], res[NV];
+template <typename T, bool Q8, int VE>
+__device__ __forceinline__ auto output(const float (&hw)[VE], float f, float pre) {
+  if constexpr (Q8) {
+    if (pre == 1.f) return encode_e4m3<VE>(hw, f);
+    float y[VE];
 #pragma unroll
-  for (int i = 0; i < NV; ++i) {
-    const int c = (i * tpr + t) * VE;
-    if (live && c < p.cols) h[i] = load_pack<T, VE>(x + c);
+    for (int j = 0; j < VE; ++j) y[j] = hw[j] * pre;
+    return encode_e4m3<VE>(y, f);
+  } else {
+    float y[VE];
+#pragma unroll
+    for (int j = 0; j < VE; ++j) y[j] = hw[j] * f;
+    return from_floats<T, VE>(y);
   }
-  if (r) {
+}
+
+// Bytes of a row that one thread holds, an element of 16 bits alone taking a register.
+template <typename T, int VE, int NV>
+constexpr int kThreadBytes = NV * (sizeof(T) * VE < 4 ? 4 : sizeof(T) * VE);
+
+// tpr threads take a row, NV vectors of VE elements each: a whole block for tpr > 32, else (a power of two)
+// one of blockDim.x / tpr groups of a block. A group walks the rows with a stride of all groups, keeps its columns' weights in
+// registers, and fetches its next row as soon as this one's h is summed, so that loads are in
+// flight during the reduction and the stores (neither where a thread holds over 64 bytes of a row).
+// SHIFT: rows start `phase` elements behind a vector's boundary, a different number from row to
+// row; the group stride is a multiple of VE rows then, so a group's rows all have the same phase.
+template <typename T, typename WT, bool Q8, int VE, int NV, bool SHIFT>
+__global__ void __launch_bounds__(512) k_rmsnorm(const NormParams p, int tpr) {
+  constexpr bool kKeep = kThreadBytes<T, VE, NV> <= 64;
+  __shared__ SumMax sm[2][32];
+  const int per_block = blockDim.x / tpr;
+  const int t = threadIdx.x % tpr;
+  const long long stride = static_cast<long long>(gridDim.x) * per_block;
+  long long row0 = static_cast<long long>(blockIdx.x) * per_block;  // of the block: its loop is uniform
+  long long row = row0 + threadIdx.x / tpr;
+  const Columns<VE, SHIFT> c(tpr, t, static_cast<int>((p.phase + row * p.ldx) & (VE - 1)), p.cols);
+  const T* x = static_cast<const T*>(p.x);
+  const T* r = static_cast<const T*>(p.res);
+  using O = std::conditional_t<Q8, uint8_t, T>;
+  Part<T, VE, NV, SHIFT> h, res;
+  Vec<WT, VE> w[kKeep ? NV : 1];
+  float w1 = 0.f;
+  auto fetch = [&](long long rw) {
+    if (rw >= p.rows) return;
+    load_row(x + rw * p.ldx, c, h);
+    if (r) load_row(r + rw * p.ldr, c, res);
+  };
+  if constexpr (kKeep) {
+    fetch(row);
 #pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      const int c = (i * tpr + t) * VE;
-      if (live && c < p.cols) res[i] = load_pack<T, VE>(r + c);
+    for (int i = 0; i < NV; ++i) w[i] = load_weight<WT, VE, SHIFT>(p.w, c, i);
+  }
+  if (SHIFT && c.single >= 0) w1 = to_f32(static_cast<const WT*>(p.w)[c.single]);
+  int half = 0;
+  for (; row0 < p.rows; row0 += stride, row += stride) {
+    const bool live = row < p.rows;
+    float hw[NV][VE], hw1 = 0.f;
+    SumMax a{0.f, 0.f};
+    if (live) {
+      if constexpr (!kKeep) fetch(row);
+      if (r) {
+#pragma unroll
+        for (int i = 0; i < NV; ++i) add_residual<T, VE>(h.v[i], res.v[i]);
+        if constexpr (SHIFT) h.one = to_f32(from_f32<T>(h.one + res.one));
+      }
+      if (p.h) store_row(static_cast<T*>(p.h) + row * p.ldh, c, h);
+#pragma unroll
+      for (int i = 0; i < NV; ++i) {
+        if constexpr (!kKeep) w[0] = load_weight<WT, VE, SHIFT>(p.w, c, i);
+        accumulate<Q8, T, WT, VE>(h.v[i], w[kKeep ? i : 0], hw[i], a);
+      }
+      if constexpr (SHIFT) {
+        hw1 = h.one * w1;
+        a.sum = fmaf(h.one, h.one, a.sum);
+        if constexpr (Q8) a.max = fmaxf(a.max, fabsf(hw1));
+      }
+      if constexpr (kKeep) fetch(row + stride);
     }
+    a = reduce_row(a, tpr, sm[half]);
+    half ^= 1;
+    if (live) {
+      float pre;
+      const float f = finish_row<Q8>(p, row, a, t == 0, pre);
+      O* y = static_cast<O*>(p.y) + row * p.ldy;
 #pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      const int c = (i * tpr + t) * VE;
-      if (live && c < p.cols) add_residual<T, VE>(h[i], res[i]);
+      for (int i = 0; i < NV; ++i)
+        if (c.has(i)) store_words<sizeof(O) * VE>(y + c.col(i), output<T, Q8, VE>(hw[i], f, pre));
+      if constexpr (SHIFT) {
+        const float one[1] = {hw1};
+        if (c.single >= 0) store_words<sizeof(O)>(y + c.single, output<T, Q8, 1>(one, f, pre));
+      }
     }
-  }
-  SumMax a{0.f, 0.f};
-#pragma unroll
-  for (int i = 0; i < NV; ++i) {
-    const int c = (i * tpr + t) * VE;
-    if (!live || c >= p.cols) continue;
-    if (p.h) store_pack<T, VE>(static_cast<T*>(p.h) + row * p.ldh + c, h[i]);
-    accumulate<T, Q8, VE>(p, c, h[i], a);
-  }
-  a = reduce_row(a, tpr, sm);
-  if (!live) return;
-  float mul;
-  const float rstd = finish_row<Q8>(p, row, a, t == 0, mul);
-#pragma unroll
-  for (int i = 0; i < NV; ++i) {
-    const int c = (i * tpr + t) * VE;
-    if (c < p.cols) write_out<T, Q8, VE>(p, row, c, h[i], rstd, mul);
   }
 }
 
 // Rows too long for the registers of one block: one block a row, which reads its row twice (the
 // second time from L2).
-template <typename T, bool Q8, int VE>
+template <typename T, typename WT, bool Q8, int VE>
 __global__ void __launch_bounds__(1024) k_rmsnorm_wide(const NormParams p) {
   __shared__ SumMax sm[32];
   const long long row = blockIdx.x;
@@ -262,27 +407,32 @@ __global__ void __launch_bounds__(1024) k_rmsnorm_wide(const NormParams p) {
   const T* r = p.res ? static_cast<const T*>(p.res) + row * p.ldr : nullptr;
   T* hr = p.h ? static_cast<T*>(p.h) + row * p.ldh : nullptr;
   SumMax a{0.f, 0.f};
+  const WT* w = static_cast<const WT*>(p.w);
+  float hw[VE];
   for (long long c = static_cast<long long>(threadIdx.x) * VE; c < p.cols; c += 1024LL * VE) {
-    Pack<T, VE> h = load_pack<T, VE>(x + c);
-    if (r) add_residual<T, VE>(h, load_pack<T, VE>(r + c));
-    if (hr) store_pack<T, VE>(hr + c, h);
-    accumulate<T, Q8, VE>(p, c, h, a);
+    Vec<T, VE> h = load_words<sizeof(T) * VE>(x + c);
+    if (r) add_residual<T, VE>(h, load_words<sizeof(T) * VE>(r + c));
+    if (hr) store_words<sizeof(T) * VE>(hr + c, h);
+    accumulate<Q8, T, WT, VE>(h, load_words<sizeof(WT) * VE>(w + c), hw, a);
   }
   a = reduce_row(a, 1024, sm);
-  float mul;
-  const float rstd = finish_row<Q8>(p, row, a, threadIdx.x == 0, mul);
+  float pre;
+  const float f = finish_row<Q8>(p, row, a, threadIdx.x == 0, pre);
   for (long long c = static_cast<long long>(threadIdx.x) * VE; c < p.cols; c += 1024LL * VE) {
     // this thread wrote h[c] itself; where h is not kept, the sum is taken again. x and the
     // residual still hold their values then: h and y are written at this thread's own columns,
     // and a column's y after its last read.
-    Pack<T, VE> h;
+    Vec<T, VE> h;
     if (hr) {
-      h = load_pack<T, VE>(hr + c);
+      h = load_words<sizeof(T) * VE>(hr + c);
     } else {
-      h = load_pack<T, VE>(x + c);
-      if (r) add_residual<T, VE>(h, load_pack<T, VE>(r + c));
+      h = load_words<sizeof(T) * VE>(x + c);
+      if (r) add_residual<T, VE>(h, load_words<sizeof(T) * VE>(r + c));
     }
-    write_out<T, Q8, VE>(p, row, c, h, rstd, mul);
+    SumMax unused{0.f, 0.f};
+    accumulate<false, T, WT, VE>(h, load_words<sizeof(WT) * VE>(w + c), hw, unused);
+    using O = std::conditional_t<Q8, uint8_t, T>;
+    store_words<sizeof(O) * VE>(static_cast<O*>(p.y) + row * p.ldy + c, output<T, Q8, VE>(hw, f, pre));
   }
 }
 
@@ -300,125 +450,142 @@ struct NormGradParams {
   long long rows;
   int cols;
   int slabs;           // blocks (each adds up the rows it takes)
+  int phase;           // elements between a vector's boundary and the first row (SHIFT)
 };
 
-// A block takes row groups blockIdx.x, + gridDim.x, ...; each thread keeps the weight gradient of
-// its own columns in registers over all of them.
-template <int VE>
-constexpr int kGradThreads = VE == 1 ? 1024 : 512;  // 64 / 128 registers a thread
-template <typename T, int VE>
-constexpr int kGradMaxNv = VE == 1 ? 16 : sizeof(T) == 4 ? 8 : 4;
-template <typename T, int VE, int NV>
-__global__ void __launch_bounds__(kGradThreads<VE>) k_rmsnorm_grad(const NormGradParams p, int tpr) {
+// Rows, columns and phases as in k_rmsnorm; each thread keeps the weight gradient of its own
+// columns in registers over all its rows. With g = dy w:
+//   dx = rstd g - h (rstd^3 / cols) sum(g h) + dresidual,   dw += (dy rstd) h
+// Where a thread holds up to 32 bytes of a row it keeps its weights and fetches the next row during this
+// one's reduction; else it reads the weights again and dresidual late.
+template <typename T, typename WT, int VE, int NV, bool SHIFT>
+__global__ void __launch_bounds__(512) k_rmsnorm_grad(const NormGradParams p, int tpr) {
+  constexpr bool kKeep = kThreadBytes<T, VE, NV> <= 32;
   __shared__ SumMax sm[2][32];
-  extern __shared__ float cols_sum[];  // tpr <= 32: [row of the block][cols]
-  const int t = threadIdx.x & (tpr - 1);
+  extern __shared__ float cols_sum[];  // tpr <= 32: [group of the block][cols]
   const int per_block = blockDim.x / tpr, mine = threadIdx.x / tpr;
+  const int t = threadIdx.x - mine * tpr;
+  const long long stride = static_cast<long long>(gridDim.x) * per_block;
+  long long row0 = static_cast<long long>(blockIdx.x) * per_block;
+  long long row = row0 + mine;
+  const Columns<VE, SHIFT> c(tpr, t, static_cast<int>((p.phase + row * p.ldh) & (VE - 1)), p.cols);
+  const T* dys = static_cast<const T*>(p.dy);
+  const T* hs = static_cast<const T*>(p.h);
+  const T* drs = static_cast<const T*>(p.dres);
   const float inv_cols = 1.f / static_cast<float>(p.cols);
-  float dw[NV][VE];
+  using Row = Part<T, VE, NV, SHIFT>;
+  Row dy, h, dr;
+  Vec<WT, VE> w[kKeep ? NV : 1];
+  float dw[NV][VE], dw1 = 0.f, w1 = 0.f;
+  float rstd = 0.f;
+  auto fetch = [&](long long rw, Row& dyv, Row& hv, Row& drv, float& rs) {
+    if (rw >= p.rows) return;
+    load_row(dys + rw * p.lddy, c, dyv);
+    load_row(hs + rw * p.ldh, c, hv);
+    if constexpr (kKeep)
+      if (drs) load_row(drs + rw * p.lddr, c, drv);
+    rs = p.rstd[rw];
+  };
+  if constexpr (kKeep) {
+    fetch(row, dy, h, dr, rstd);
+#pragma unroll
+    for (int i = 0; i < NV; ++i) w[i] = load_weight<WT, VE, SHIFT>(p.w, c, i);
+  }
+  if (SHIFT && c.single >= 0) w1 = to_f32(static_cast<const WT*>(p.w)[c.single]);
 #pragma unroll
   for (int i = 0; i < NV; ++i)
 #pragma unroll
     for (int j = 0; j < VE; ++j) dw[i][j] = 0.f;
   int half = 0;
-  for (long long r0 = static_cast<long long>(blockIdx.x) * per_block; r0 < p.rows;
-       r0 += static_cast<long long>(gridDim.x) * per_block) {
-    const long long row = r0 + mine;
+  for (; row0 < p.rows; row0 += stride, row += stride) {
     const bool live = row < p.rows;
-    const T* dyr = static_cast<const T*>(p.dy) + row * p.lddy;
-    const T* hr = static_cast<const T*>(p.h) + row * p.ldh;
-    Pack<T, VE> dy[NV], h[NV];
-#pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      const int c = (i * tpr + t) * VE;
-      if (live && c < p.cols) {
-        dy[i] = load_pack<T, VE>(dyr + c);
-        h[i] = load_pack<T, VE>(hr + c);
-      }
+    Row dy2, h2, dr2;
+    float rstd2 = 0.f;
+    if (live) {
+      if constexpr (kKeep) fetch(row + stride, dy2, h2, dr2, rstd2);
+      else fetch(row, dy, h, dr, rstd);
     }
-    const float rstd = live ? p.rstd[row] : 0.f;
     SumMax a{0.f, 0.f};
+    if (live) {
 #pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      const int c = (i * tpr + t) * VE;
-      if (!live || c >= p.cols) continue;
-      float w[VE];
-      load_weight<T, VE>(p.w, p.w_f32, c, w);
+      for (int i = 0; i < NV; ++i) {
+        if constexpr (!kKeep) w[0] = load_weight<WT, VE, SHIFT>(p.w, c, i);
 #pragma unroll
-      for (int j = 0; j < VE; ++j) {
-        const float n = to_f32(h[i].v[j]) * rstd, d = to_f32(dy[i].v[j]);
-        a.sum = fmaf(d * w[j], n, a.sum);
-        dw[i][j] = fmaf(d, n, dw[i][j]);
+        for (int j = 0; j < VE; ++j) {
+          const float d = elem<T>(dy.v[i], j), v = elem<T>(h.v[i], j);
+          a.sum = fmaf(d * elem<WT>(w[kKeep ? i : 0], j), v, a.sum);
+          dw[i][j] = fmaf(d * rstd, v, dw[i][j]);
+        }
+      }
+      if constexpr (SHIFT) {
+        a.sum = fmaf(dy.one * w1, h.one, a.sum);
+        dw1 = fmaf(dy.one * rstd, h.one, dw1);
       }
     }
     a = reduce_row(a, tpr, sm[half]);
     half ^= 1;
-    const float mean = a.sum * inv_cols;
+    if (live) {
+      const float coef = rstd * rstd * rstd * (a.sum * inv_cols);
+      if constexpr (!kKeep)
+        if (drs) load_row(drs + row * p.lddr, c, dr);
 #pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      const int c = (i * tpr + t) * VE;
-      if (!live || c >= p.cols) continue;
-      float w[VE];
-      load_weight<T, VE>(p.w, p.w_f32, c, w);
-      Pack<T, VE> o, dr;
-      if (p.dres) dr = load_pack<T, VE>(static_cast<const T*>(p.dres) + row * p.lddr + c);
+      for (int i = 0; i < NV; ++i) {
+        if constexpr (!kKeep) w[0] = load_weight<WT, VE, SHIFT>(p.w, c, i);
+        float o[VE];
 #pragma unroll
-      for (int j = 0; j < VE; ++j) {
-        const float n = to_f32(h[i].v[j]) * rstd;
-        float g = rstd * (to_f32(dy[i].v[j]) * w[j] - n * mean);
-        if (p.dres) g += to_f32(dr.v[j]);
-        o.v[j] = from_f32<T>(g);
+        for (int j = 0; j < VE; ++j) {
+          o[j] = elem<T>(dy.v[i], j) * elem<WT>(w[kKeep ? i : 0], j) * rstd - elem<T>(h.v[i], j) * coef;
+          if (drs) o[j] += elem<T>(dr.v[i], j);
+        }
+        dy.v[i] = from_floats<T, VE>(o);
       }
-      store_pack<T, VE>(static_cast<T*>(p.dx) + row * p.lddx + c, o);
+      if constexpr (SHIFT) {
+        dy.one = dy.one * w1 * rstd - h.one * coef;
+        if (drs) dy.one += dr.one;
+      }
+      store_row(static_cast<T*>(p.dx) + row * p.lddx, c, dy);
+      if constexpr (kKeep) {
+        dy = dy2;
+        h = h2;
+        dr = dr2;
+        rstd = rstd2;
+      }
     }
   }
   float* out = p.partial + static_cast<long long>(blockIdx.x) * p.cols;
-  if (tpr > 32) {
+  float* mine_out = tpr > 32 ? out : cols_sum + mine * p.cols;
 #pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      const int c = (i * tpr + t) * VE;
-      if (c >= p.cols) continue;
+  for (int i = 0; i < NV; ++i)
+    if (c.has(i)) {
 #pragma unroll
-      for (int j = 0; j < VE; ++j) out[c + j] = dw[i][j];
+      for (int j = 0; j < VE; ++j) mine_out[c.col(i) + j] = dw[i][j];
     }
-    return;
-  }
-#pragma unroll
-  for (int i = 0; i < NV; ++i) {
-    const int c = (i * tpr + t) * VE;
-    if (c >= p.cols) continue;
-#pragma unroll
-    for (int j = 0; j < VE; ++j) cols_sum[mine * p.cols + c + j] = dw[i][j];
-  }
+  if (SHIFT && c.single >= 0) mine_out[c.single] = dw1;
+  if (tpr > 32) return;
   __syncthreads();
-  for (int c = threadIdx.x; c < p.cols; c += blockDim.x) {
+  for (int j = threadIdx.x; j < p.cols; j += blockDim.x) {
     float s = 0.f;
-    for (int g = 0; g < per_block; ++g) s += cols_sum[g * p.cols + c];
-    out[c] = s;
+    for (int g = 0; g < per_block; ++g) s += cols_sum[g * p.cols + j];
+    out[j] = s;
   }
 }
 
 // Rows too long for registers: dx with the row read twice, and the weight gradient's slabs by
 // columns in a kernel of their own.
-template <typename T>
+template <typename T, typename WT>
 __global__ void __launch_bounds__(1024) k_rmsnorm_grad_wide(const NormGradParams p) {
   __shared__ SumMax sm[32];
   const long long row = blockIdx.x;
   const T* dy = static_cast<const T*>(p.dy) + row * p.lddy;
   const T* h = static_cast<const T*>(p.h) + row * p.ldh;
+  const WT* w = static_cast<const WT*>(p.w);
   const float rstd = p.rstd[row];
   SumMax a{0.f, 0.f};
-  for (long long c = threadIdx.x; c < p.cols; c += 1024) {
-    float w[1];
-    load_weight<T, 1>(p.w, p.w_f32, c, w);
-    a.sum = fmaf(to_f32(dy[c]) * w[0], to_f32(h[c]) * rstd, a.sum);
-  }
+  for (long long c = threadIdx.x; c < p.cols; c += 1024) a.sum = fmaf(to_f32(dy[c]) * to_f32(w[c]), to_f32(h[c]), a.sum);
   a = reduce_row(a, 1024, sm);
-  const float mean = a.sum / static_cast<float>(p.cols);
+  const float coef = rstd * rstd * rstd * (a.sum / static_cast<float>(p.cols));
   for (long long c = threadIdx.x; c < p.cols; c += 1024) {
-    float w[1];
-    load_weight<T, 1>(p.w, p.w_f32, c, w);
-    float g = rstd * (to_f32(dy[c]) * w[0] - to_f32(h[c]) * rstd * mean);
+    float g = to_f32(dy[c]) * to_f32(w[c]) * rstd - to_f32(h[c]) * coef;
     if (p.dres) g += to_f32(static_cast<const T*>(p.dres)[row * p.lddr + c]);
     static_cast<T*>(p.dx)[row * p.lddx + c] = from_f32<T>(g);
   }
@@ -430,8 +597,8 @@ __global__ void __launch_bounds__(256) k_rmsnorm_dw_wide(const NormGradParams p)
   for (int slab = blockIdx.y; slab < p.slabs; slab += gridDim.y) {
     float s = 0.f;
     for (long long row = slab; row < p.rows; row += p.slabs)
-      s = fmaf(to_f32(static_cast<const T*>(p.dy)[row * p.lddy + c]),
-               to_f32(static_cast<const T*>(p.h)[row * p.ldh + c]) * p.rstd[row], s);
+      s = fmaf(to_f32(static_cast<const T*>(p.dy)[row * p.lddy + c]) * p.rstd[row],
+               to_f32(static_cast<const T*>(p.h)[row * p.ldh + c]), s);
     p.partial[static_cast<long long>(slab) * p.cols + c] = s;
   }
 }
@@ -459,59 +626,118 @@ int elem_bytes(int dtype) { return dtype == BW_DTYPE_F32 ? 4 : 2; }
 
 bool norm_dtype_ok(int dtype) { return dtype == BW_DTYPE_F32 || dtype == BW_DTYPE_F16 || dtype == BW_DTYPE_BF16; }
 
-bool multiple_of(const void* p, long long ld, int elem, int bytes) {
-  return (reinterpret_cast<uintptr_t>(p) % bytes) == 0 && (ld * elem) % bytes == 0;
-}
-
 struct Shape {
   int tpr, nv;  // nv = 0: too long for registers
+  int block;
+  long long groups;  // a block
 };
 
-// Threads a row and vectors a thread: NV vectors a thread where there are rows enough to fill the
-// GPU, more threads and fewer vectors otherwise (each load waits once, so a short chain per thread).
-Shape row_shape(long long rows, int cols, int ve, int max_tpr, int max_nv) {
-  const long long nvec = (static_cast<long long>(cols) + ve - 1) / ve;
-  const int want = rows >= 1024 ? 4 : 1;
-  int tpr = 1;
-  while (tpr < max_tpr && static_cast<long long>(tpr) * want < nvec) tpr *= 2;
-  int nv = 1;
-  while (nv <= max_nv && static_cast<long long>(nv) * tpr < nvec) nv *= 2;
-  if (nv > max_nv) nv = 0;
-  return {tpr, nv};
+// Threads a row (at least min_tpr) and vectors a thread (1, 2, 4, ... up to max_nv). Few rows: a vector a thread (each load
+// waits once). Many: `want` vectors, so that a block is small and each thread has more loads in flight;
+// fewer where a warp's granularity would leave over an eighth more of them idle.
+constexpr int kMaxThreads = 512;
+Shape row_shape(long long rows, long long nvec, int want, int max_nv, int min_tpr) {
+  if (rows < 512) want = 1;
+  int nv = want;
+  while (nv <= max_nv && nvec > static_cast<long long>(nv) * kMaxThreads) nv *= 2;
+  if (nv > max_nv) return {0, 0, 0, 0};
+  if (nvec <= 32 * nv) {  // groups inside warps
+    int tpr = min_tpr;
+    while (tpr * nv < nvec) tpr *= 2;
+    return {tpr, nv, 256, 256 / tpr};
+  }
+  auto threads = [&](int n) { return static_cast<int>((nvec + 32 * n - 1) / (32 * n)) * 32; };
+  for (int n = nv / 2; n >= 1 && threads(n) <= kMaxThreads; n /= 2)
+    if (8 * threads(nv) * nv > 9 * threads(n) * n) nv = n;
+  return {threads(nv), nv, threads(nv), 1};
 }
 
-template <typename T, bool Q8, int VE>
-int launch_norm(const NormParams& p, cudaStream_t s) {
-  const Shape sh = row_shape(p.rows, p.cols, VE, 1024, VE == 1 ? 8 : 4);
-  const int block = sh.tpr > 32 ? sh.tpr : 256;
-  const long long per = block / sh.tpr;
-  const long long grid = (p.rows + per - 1) / per;
-  if (sh.nv == 0) {
-    k_rmsnorm_wide<T, Q8, VE><<<static_cast<unsigned>(p.rows), 1024, 0, s>>>(p);
-  } else {
-    const unsigned g = static_cast<unsigned>(grid);
-    switch (sh.nv) {
-      case 1: k_rmsnorm<T, Q8, VE, 1><<<g, block, 0, s>>>(p, sh.tpr); break;
-      case 2: k_rmsnorm<T, Q8, VE, 2><<<g, block, 0, s>>>(p, sh.tpr); break;
-      case 4: k_rmsnorm<T, Q8, VE, 4><<<g, block, 0, s>>>(p, sh.tpr); break;
-      default:
-        if constexpr (VE == 1) k_rmsnorm<T, Q8, 1, 8><<<g, block, 0, s>>>(p, sh.tpr);
-        break;
-    }
+// How a call's rows are read: 16-byte vectors from a boundary, vectors behind one (every tensor's
+// row at the same distance, which contiguous tensors have whatever cols is), or element by element.
+enum class Access { ALIGNED, SHIFTED, SCALAR };
+struct RowsOf {  // one tensor: address, pitch in elements, element size
+  const void* p;
+  long long ld;
+  int elem;
+};
+template <int N>
+Access row_access(const RowsOf (&t)[N], int ve, long long cols, int* phase) {
+  // element offset from a vector's boundary of the tensor's first row
+  auto first = [&](const RowsOf& o) { return static_cast<long long>(reinterpret_cast<uintptr_t>(o.p) / o.elem % ve); };
+  const RowsOf& a = t[0];
+  bool same = true, aligned = cols % ve == 0;
+  for (const RowsOf& o : t) {
+    if (!o.p) continue;
+    same = same && first(o) == first(a) && (o.ld - a.ld) % ve == 0;
+    aligned = aligned && first(o) == 0 && o.ld % ve == 0;
   }
+  *phase = static_cast<int>(first(a));
+  return aligned ? Access::ALIGNED : same ? Access::SHIFTED : Access::SCALAR;
+}
+
+// As many blocks as are resident at once (16384 x 8192 BF16: 141 us; with one more a SM 143 us, and with
+// a few left over twice as long), each with its share of the rows.
+template <typename Kernel>
+int launch_rows(Kernel kern, const NormParams& p, const Shape& sh, bool shift, cudaStream_t s, const DeviceState& d) {
+  static std::atomic<int> resident[kMaxThreads / 32 + 1] = {};  // by block size, of this kernel; 0: not asked yet
+  std::atomic<int>& known = resident[sh.block / 32];
+  int per_sm = known.load(std::memory_order_relaxed);
+  if (per_sm == 0) {
+    BW_CUDA(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kern, sh.block, 0));
+    known.store(per_sm, std::memory_order_relaxed);
+  }
+  long long grid = (p.rows + sh.groups - 1) / sh.groups;
+  long long cap = static_cast<long long>(d.sms) * per_sm;
+  if (shift) cap = cap / 8 * 8;  // a stride of whole phases
+  if (grid > cap) grid = cap;
+  kern<<<static_cast<unsigned>(grid), sh.block, 0, s>>>(p, sh.tpr);
   BW_CUDA(cudaGetLastError());
   return BW_OK;
 }
 
-template <typename T, bool Q8>
-int dispatch_norm(const NormParams& p, cudaStream_t s) {
+template <typename T, typename WT, bool Q8, int VE, bool SHIFT>
+int launch_norm(const NormParams& p, cudaStream_t s, const DeviceState& d) {
+  constexpr int kMaxNv = VE == 1 ? 16 : sizeof(T) == 4 ? 8 : 4;
+  const long long nvec = SHIFT ? p.cols / VE : (p.cols + VE - 1LL) / VE;
+  const Shape sh = row_shape(p.rows, nvec, 4, kMaxNv, SHIFT ? 16 : 1);
+  if (sh.nv == 0) {
+    constexpr int WVE = SHIFT ? 1 : VE;
+    k_rmsnorm_wide<T, WT, Q8, WVE><<<static_cast<unsigned>(p.rows), 1024, 0, s>>>(p);
+    BW_CUDA(cudaGetLastError());
+    return BW_OK;
+  }
+  switch (sh.nv) {
+    case 1: return launch_rows(k_rmsnorm<T, WT, Q8, VE, 1, SHIFT>, p, sh, SHIFT, s, d);
+    case 2: return launch_rows(k_rmsnorm<T, WT, Q8, VE, 2, SHIFT>, p, sh, SHIFT, s, d);
+    case 4: return launch_rows(k_rmsnorm<T, WT, Q8, VE, 4, SHIFT>, p, sh, SHIFT, s, d);
+    case 8:
+      if constexpr (kMaxNv >= 8) return launch_rows(k_rmsnorm<T, WT, Q8, VE, 8, SHIFT>, p, sh, SHIFT, s, d);
+      [[fallthrough]];
+    default:
+      if constexpr (kMaxNv >= 16) return launch_rows(k_rmsnorm<T, WT, Q8, VE, 16, SHIFT>, p, sh, SHIFT, s, d);
+      return BW_OK;  // row_shape gives no more than kMaxNv
+  }
+}
+
+template <typename T, typename WT, bool Q8>
+int dispatch_norm(NormParams p, cudaStream_t s, const DeviceState& d) {
   constexpr int VE = 16 / sizeof(T);
   const int e = sizeof(T);
-  // 16-byte vectors need every row of every tensor to start on its vector's boundary
-  const bool vec = p.cols % VE == 0 && multiple_of(p.x, p.ldx, e, 16) && (!p.res || multiple_of(p.res, p.ldr, e, 16)) &&
-                   (!p.h || multiple_of(p.h, p.ldh, e, 16)) && multiple_of(p.y, p.ldy, Q8 ? 1 : e, Q8 ? VE : 16) &&
-                   multiple_of(p.w, 0, 1, 16);
-  return vec ? launch_norm<T, Q8, VE>(p, s) : launch_norm<T, Q8, 1>(p, s);
+  const RowsOf t[] = {{p.x, p.ldx, e}, {p.res, p.ldr, e}, {p.h, p.ldh, e}, {p.y, p.ldy, Q8 ? 1 : e}};
+  switch (row_access(t, VE, p.cols, &p.phase)) {
+    case Access::ALIGNED:
+      if (aligned16(p.w)) return launch_norm<T, WT, Q8, VE, false>(p, s, d);
+      [[fallthrough]];
+    case Access::SHIFTED: return launch_norm<T, WT, Q8, VE, true>(p, s, d);
+    default: return launch_norm<T, WT, Q8, 1, false>(p, s, d);
+  }
+}
+
+template <typename T>
+int dispatch_weight(const NormParams& p, bool q8, cudaStream_t s, const DeviceState& d) {
+  if constexpr (sizeof(T) < 4)
+    if (p.w_f32) return q8 ? dispatch_norm<T, float, true>(p, s, d) : dispatch_norm<T, float, false>(p, s, d);
+  return q8 ? dispatch_norm<T, T, true>(p, s, d) : dispatch_norm<T, T, false>(p, s, d);
 }
 
 int check_pitch(const char* what, long long ld, long long rows, int cols) {
@@ -572,39 +798,47 @@ int norm_impl(const void* x, long long ldx, const void* residual, long long ldr,
   p.cols = cols;
   p.eps = eps;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  if (dtype == BW_DTYPE_F32) return q8 ? dispatch_norm<float, true>(p, s) : dispatch_norm<float, false>(p, s);
-  if (dtype == BW_DTYPE_F16) return q8 ? dispatch_norm<__half, true>(p, s) : dispatch_norm<__half, false>(p, s);
-  return q8 ? dispatch_norm<__nv_bfloat16, true>(p, s) : dispatch_norm<__nv_bfloat16, false>(p, s);
+  if (dtype == BW_DTYPE_F32) return dispatch_weight<float>(p, q8, s, *d);
+  if (dtype == BW_DTYPE_F16) return dispatch_weight<__half>(p, q8, s, *d);
+  return dispatch_weight<__nv_bfloat16>(p, q8, s, *d);
 }
 
-// Slabs of the weight gradient: a function of the sizes alone, so that the sums (and the
-// workspace) are the same on every device.
-constexpr int kMaxSlabs = 296;
-int grad_slabs(long long rows) { return static_cast<int>(rows < kMaxSlabs ? rows : kMaxSlabs); }
+// Slabs of the weight gradient, one a block: a function of the sizes alone, so that the sums (and the
+// workspace) are the same on every device. 512 threads are resident on an SM (of 148) with this
+// kernel's registers, and a block has one for 16 columns, or 256 for short rows; more slabs wait for a
+// second round and write more partial sums (16384 x 8192 BF16: 180 us with 148, 185 with 296, 199 with 592).
+int grad_slabs(long long rows, long long cols) {
+  long long most = 296;
+  if (cols > 512 && cols <= 16384) most = 148LL * 512 / (cols > 8192 ? 512 : (cols + 511) / 512 * 32);
+  if (cols <= 16384 && most > rows / 4) most = rows / 4 > 148 ? rows / 4 : 148;
+  return static_cast<int>(rows < most ? rows : most);
+}
 
-template <typename T, int VE>
+template <typename T, typename WT, int VE, bool SHIFT>
 int launch_grad(NormGradParams p, float* dw, cudaStream_t s) {
-  const Shape sh = row_shape(p.rows, p.cols, VE, kGradThreads<VE>, kGradMaxNv<T, VE>);
+  constexpr int kMaxNv = VE == 1 ? 16 : sizeof(T) == 4 ? 8 : 4;
+  const long long nvec = SHIFT ? p.cols / VE : (p.cols + VE - 1LL) / VE;
+  // 32 bytes of a row a thread (it fetches ahead then), 64 for long sums in FP32
+  const Shape sh = row_shape(p.rows, nvec, sizeof(T) == 4 && p.rows >= 2048 ? 4 : 2, kMaxNv, SHIFT ? 16 : 1);
   if (sh.nv == 0) {
     // the weight gradient first: dx may be written over dy or h
     k_rmsnorm_dw_wide<T><<<dim3(static_cast<unsigned>((p.cols + 255LL) / 256), p.slabs), 256, 0, s>>>(p);
     BW_CUDA(cudaGetLastError());
-    k_rmsnorm_grad_wide<T><<<static_cast<unsigned>(p.rows), 1024, 0, s>>>(p);
+    k_rmsnorm_grad_wide<T, WT><<<static_cast<unsigned>(p.rows), 1024, 0, s>>>(p);
   } else {
-    const int block = sh.tpr > 32 ? sh.tpr : 256;
-    const long long per = block / sh.tpr;
-    const long long groups = (p.rows + per - 1) / per;
-    if (groups < p.slabs) p.slabs = static_cast<int>(groups);
-    const size_t smem = sh.tpr > 32 ? 0 : static_cast<size_t>(per) * p.cols * sizeof(float);
+    const long long groups = (p.rows + sh.groups - 1) / sh.groups;
+    if (groups <= p.slabs) p.slabs = static_cast<int>(groups);  // a row each
+    else if (SHIFT && sh.groups < 8) p.slabs = p.slabs / 8 * 8;  // a stride of whole phases
+    const size_t smem = sh.tpr > 32 ? 0 : static_cast<size_t>(sh.groups) * p.cols * sizeof(float);
     switch (sh.nv) {
-      case 1: k_rmsnorm_grad<T, VE, 1><<<p.slabs, block, smem, s>>>(p, sh.tpr); break;
-      case 2: k_rmsnorm_grad<T, VE, 2><<<p.slabs, block, smem, s>>>(p, sh.tpr); break;
-      case 4: k_rmsnorm_grad<T, VE, 4><<<p.slabs, block, smem, s>>>(p, sh.tpr); break;
+      case 1: k_rmsnorm_grad<T, WT, VE, 1, SHIFT><<<p.slabs, sh.block, smem, s>>>(p, sh.tpr); break;
+      case 2: k_rmsnorm_grad<T, WT, VE, 2, SHIFT><<<p.slabs, sh.block, smem, s>>>(p, sh.tpr); break;
+      case 4: k_rmsnorm_grad<T, WT, VE, 4, SHIFT><<<p.slabs, sh.block, smem, s>>>(p, sh.tpr); break;
       case 8:
-        if constexpr (kGradMaxNv<T, VE> >= 8) k_rmsnorm_grad<T, VE, 8><<<p.slabs, block, smem, s>>>(p, sh.tpr);
+        if constexpr (kMaxNv >= 8) k_rmsnorm_grad<T, WT, VE, 8, SHIFT><<<p.slabs, sh.block, smem, s>>>(p, sh.tpr);
         break;
       default:
-        if constexpr (kGradMaxNv<T, VE> >= 16) k_rmsnorm_grad<T, VE, 16><<<p.slabs, block, smem, s>>>(p, sh.tpr);
+        if constexpr (kMaxNv >= 16) k_rmsnorm_grad<T, WT, VE, 16, SHIFT><<<p.slabs, sh.block, smem, s>>>(p, sh.tpr);
         break;
     }
   }
@@ -614,14 +848,25 @@ int launch_grad(NormGradParams p, float* dw, cudaStream_t s) {
   return BW_OK;
 }
 
-template <typename T>
-int dispatch_grad(const NormGradParams& p, float* dw, cudaStream_t s) {
+template <typename T, typename WT>
+int dispatch_grad(NormGradParams p, float* dw, cudaStream_t s) {
   constexpr int VE = 16 / sizeof(T);
   const int e = sizeof(T);
-  const bool vec = p.cols % VE == 0 && multiple_of(p.dy, p.lddy, e, 16) && multiple_of(p.h, p.ldh, e, 16) &&
-                   (!p.dres || multiple_of(p.dres, p.lddr, e, 16)) && multiple_of(p.dx, p.lddx, e, 16) &&
-                   multiple_of(p.w, 0, 1, 16);
-  return vec ? launch_grad<T, VE>(p, dw, s) : launch_grad<T, 1>(p, dw, s);
+  const RowsOf t[] = {{p.h, p.ldh, e}, {p.dy, p.lddy, e}, {p.dres, p.lddr, e}, {p.dx, p.lddx, e}};
+  switch (row_access(t, VE, p.cols, &p.phase)) {
+    case Access::ALIGNED:
+      if (aligned16(p.w)) return launch_grad<T, WT, VE, false>(p, dw, s);
+      [[fallthrough]];
+    case Access::SHIFTED: return launch_grad<T, WT, VE, true>(p, dw, s);
+    default: return launch_grad<T, WT, 1, false>(p, dw, s);
+  }
+}
+
+template <typename T>
+int dispatch_grad_weight(const NormGradParams& p, float* dw, cudaStream_t s) {
+  if constexpr (sizeof(T) < 4)
+    if (p.w_f32) return dispatch_grad<T, float>(p, dw, s);
+  return dispatch_grad<T, T>(p, dw, s);
 }
 
 }  // namespace
@@ -647,7 +892,7 @@ int bw_rmsnorm_fp8(const void* x, long long ldx, const void* residual, long long
 
 size_t bw_rmsnorm_backward_workspace(int rows, int cols) {
   if (rows <= 0 || cols <= 0) return 0;
-  return static_cast<size_t>(grad_slabs(rows)) * cols * sizeof(float);
+  return static_cast<size_t>(grad_slabs(rows, cols)) * cols * sizeof(float);
 }
 
 int bw_rmsnorm_backward(const void* dy, long long lddy, const void* h, long long ldh, const void* weight, int dtype,
@@ -695,10 +940,10 @@ int bw_rmsnorm_backward(const void* dy, long long lddy, const void* h, long long
   p.lddx = lddx;
   p.rows = rows;
   p.cols = cols;
-  p.slabs = grad_slabs(rows);
-  if (dtype == BW_DTYPE_F32) return dispatch_grad<float>(p, dweight, s);
-  if (dtype == BW_DTYPE_F16) return dispatch_grad<__half>(p, dweight, s);
-  return dispatch_grad<__nv_bfloat16>(p, dweight, s);
+  p.slabs = grad_slabs(rows, cols);
+  if (dtype == BW_DTYPE_F32) return dispatch_grad_weight<float>(p, dweight, s);
+  if (dtype == BW_DTYPE_F16) return dispatch_grad_weight<__half>(p, dweight, s);
+  return dispatch_grad_weight<__nv_bfloat16>(p, dweight, s);
 }
 
 }  // extern "C"
