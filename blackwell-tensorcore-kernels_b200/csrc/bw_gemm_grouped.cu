@@ -106,14 +106,19 @@ int launch(const Operands& o, int dtype, GroupedParams p, cudaStream_t s, const 
     clusters[dev & 63] = pair_clusters_resident(
         two, kGroupedThreads, kPairStages * kPairStageBytes + grouped_tail_bytes(kMaxGroups), d);
   }
-  if (pair) {
-    const int n = static_cast<int>(most < clusters[dev & 63] ? most : clusters[dev & 63]);
-    two<<<2 * n, kGroupedThreads, smem, s>>>(ta, ta16, tb, p);
-  } else {
-    const int n = static_cast<int>(most < d.sms ? most : d.sms);
-    one<<<n, kGroupedThreads, smem, s>>>(ta, ta16, tb, p);
-  }
-  BW_CUDA(cudaGetLastError());
+  const long long room = pair ? clusters[dev & 63] : d.sms;
+  const int n = static_cast<int>(most < room ? most : room);
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(pair ? 2 * n : n);
+  cfg.blockDim = dim3(kGroupedThreads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = s;
+  cudaLaunchAttribute attr = {};
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;  // see grid_dependency_wait
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  BW_CUDA(cudaLaunchKernelEx(&cfg, pair ? two : one, ta, ta16, tb, p));
   return BW_OK;
 }
 

@@ -91,6 +91,14 @@ __device__ __forceinline__ void mbar_drain(uint64_t* bar, uint32_t parity, uint6
   }
 }
 
+// Programmatic dependent launch: a grid may start while the one before it in the stream ends, and
+// waits here for that one's end (and its writes) before it touches global memory; it lets the next
+// grid start the same way. Barriers, Tensor Memory and descriptors are set up in the meantime.
+__device__ __forceinline__ void grid_dependency_wait() {
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+}
+
 // bounds[g] = first row of group g (bounds[groups] = end of the last), clamped and made
 // non-decreasing; tiles[g] = output tiles of the groups before g, `per_row` of them per tm rows.
 // All threads fetch the offsets (one trip to memory); warp 2 scans them.
@@ -331,6 +339,7 @@ __global__ void __launch_bounds__(kGroupedThreads, 1)
   // nothing is loaded (and the maps are empty) where nothing is summed
   if (warp == 0 && lane == 0 && (MODE == GMode::WGRAD ? p.rows : p.k) > 0) { tma_prefetch_desc(&tmA); tma_prefetch_desc(&tmB); }
   if (warp == 1) { tmem_alloc(tmem_slot, 512); tmem_relinquish(); }
+  grid_dependency_wait();
   grouped_fetch(p.offsets, p.groups, p.rows, bounds);
   __syncthreads();
   if (warp == 2) grouped_scan(p.groups, kBM, (p.n + p.W - 1) / p.W, bounds, MODE == GMode::WGRAD ? nullptr : tiles);
@@ -595,6 +604,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGroupedThreads, 1)
   }
   if (warp == 0 && lane == 0 && (MODE == GMode::WGRAD ? p.rows : p.k) > 0) { tma_prefetch_desc(&tmA); tma_prefetch_desc(&tmB); }
   if (warp == 1) { tmem_alloc_pair(tmem_slot, 512); tmem_relinquish_pair(); }
+  grid_dependency_wait();
   grouped_fetch(p.offsets, p.groups, p.rows, bounds);
   __syncthreads();
   if (warp == 2) grouped_scan(p.groups, 256, (p.n + 255) / 256, bounds, MODE == GMode::WGRAD ? nullptr : tiles);
