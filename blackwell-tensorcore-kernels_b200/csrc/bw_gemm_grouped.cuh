@@ -36,6 +36,7 @@ struct GroupedParams {
   int rows;                  // rows of A (X, Y)
   int m, n, k;               // WGRAD: m x n outputs a group; else n columns, k summed
   int W;                     // tile width
+  int sub;                   // K atoms a stage (single-CTA kernel)
   int stages, stage_bytes;
   int group_m;               // raster: tile rows a band
   int vec;                   // store width in bytes: 16, or the element's
@@ -300,9 +301,11 @@ template <Kind KIND, GMode MODE, Out OUT>
 __global__ void __launch_bounds__(kGroupedThreads, 1)
     bw_tc_gemm_grouped_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmA16,
                               const __grid_constant__ CUtensorMap tmB, const GroupedParams p) {
-  constexpr int KE = KindTraits<KIND>::kElemsPerSlab;   // K elements a slab (WGRAD: rows)
+  constexpr int KA = KindTraits<KIND>::kElemsPerSlab;   // K elements a swizzle atom (WGRAD: rows)
+  const int KE = KA * p.sub;                            // ... a stage
   constexpr bool A_MN = MODE == GMode::WGRAD, B_MN = MODE != GMode::ROWS_NK;
-  constexpr int kABytes = kBM * kSlabBytes;
+  constexpr int kABytes = kBM * kSlabBytes;             // an atom of A
+  const int b_bytes = p.W * kSlabBytes;                 // an atom of B
   constexpr int kBoxBytes = 64 * kSlabBytes;            // one 64 x 64 box of an MN-major operand
   static_assert(KIND == Kind::F16 || (KIND == Kind::F8 && MODE == GMode::ROWS_NK), "8-bit operands are K-contiguous");
   extern __shared__ uint8_t smem_raw[];
@@ -365,12 +368,14 @@ __global__ void __launch_bounds__(kGroupedThreads, 1)
         for (int kb = 0; kb < nk; ++kb) {
           if (!mbar_poll(&empty[s], ph ^ 1, wc, 21)) { ok = false; break; }
           uint8_t* sA = smem + static_cast<size_t>(s) * p.stage_bytes;
-          uint8_t* sB = sA + kABytes;
+          uint8_t* sB = sA + p.sub * kABytes;
+          const int left = o.k - kb * KE;
+          const int atoms = left > KA ? p.sub : 1;  // the others lie behind the end
           if constexpr (A_MN) {
             // A cut slab lands on a barrier of its own, which the tail warp waits for: it follows
             // only these (on full[s] it could fall two phases behind). full[s] completes at once.
             uint64_t* bar = &full[s];
-            if (slab_is_cut(o.k - kb * KE, KE)) {
+            if (slab_is_cut(left, KE)) {
               mbar_arrive(bar);
               bar = &tailfull[s];
               cut_last |= 1u << s;
@@ -378,24 +383,30 @@ __global__ void __launch_bounds__(kGroupedThreads, 1)
             } else {
               cut_last &= ~(1u << s);
             }
-            mbar_arrive_expect_tx(bar, p.stage_bytes);
-            tma_load_2d(&tmA, bar, sA, o.row0, o.kbase + kb * KE, pol);
-            tma_load_2d(&tmA, bar, sA + kBoxBytes, o.row0 + 64, o.kbase + kb * KE, pol);
-            for (int j = 0; j < p.W / 64; ++j)
-              tma_load_2d(&tmB, bar, sB + j * kBoxBytes, o.col0 + 64 * j, o.kbase + kb * KE, pol);
-          } else {
-            mbar_arrive_expect_tx(&full[s], a_load_bytes(o.rows) + p.W * kSlabBytes);
-            if (o.rows > kFewRows) {
-              tma_load_2d(&tmA, &full[s], sA, kb * KE, o.row0, pol);
-            } else {
-              for (int r = 0; r < o.rows; r += 16)
-                tma_load_2d(&tmA16, &full[s], sA + r * kSlabBytes, kb * KE, o.row0 + r, pol);
-            }
-            if constexpr (B_MN) {
+            mbar_arrive_expect_tx(bar, atoms * (kABytes + b_bytes));
+            for (int a = 0; a < atoms; ++a) {
+              const int y = o.kbase + kb * KE + a * KA;
+              tma_load_2d(&tmA, bar, sA + a * kABytes, o.row0, y, pol);
+              tma_load_2d(&tmA, bar, sA + a * kABytes + kBoxBytes, o.row0 + 64, y, pol);
               for (int j = 0; j < p.W / 64; ++j)
-                tma_load_3d(&tmB, &full[s], sB + j * kBoxBytes, o.col0 + 64 * j, kb * KE, o.g, pol);
-            } else {
-              tma_load_3d(&tmB, &full[s], sB, kb * KE, o.col0, o.g, pol);
+                tma_load_2d(&tmB, bar, sB + a * b_bytes + j * kBoxBytes, o.col0 + 64 * j, y, pol);
+            }
+          } else {
+            mbar_arrive_expect_tx(&full[s], atoms * (a_load_bytes(o.rows) + b_bytes));
+            for (int a = 0; a < atoms; ++a) {
+              const int x = kb * KE + a * KA;
+              if (o.rows > kFewRows) {
+                tma_load_2d(&tmA, &full[s], sA + a * kABytes, x, o.row0, pol);
+              } else {
+                for (int r = 0; r < o.rows; r += 16)
+                  tma_load_2d(&tmA16, &full[s], sA + a * kABytes + r * kSlabBytes, x, o.row0 + r, pol);
+              }
+              if constexpr (B_MN) {
+                for (int j = 0; j < p.W / 64; ++j)
+                  tma_load_3d(&tmB, &full[s], sB + a * b_bytes + j * kBoxBytes, o.col0 + 64 * j, x, o.g, pol);
+              } else {
+                tma_load_3d(&tmB, &full[s], sB + a * b_bytes, x, o.col0, o.g, pol);
+              }
             }
           }
           ++issued;
@@ -429,27 +440,25 @@ __global__ void __launch_bounds__(kGroupedThreads, 1)
         const uint32_t d_tmem = tmem_base + b * 256;
         for (int kb = 0; kb < nk; ++kb) {
           if (!mbar_poll(&full[s], ph, wc, 23)) { ok = false; break; }
-          int steps = 4;
-          if constexpr (MODE == GMode::WGRAD) {
-            const int left = o.k - kb * KE;
-            if (left < KE) {
-              steps = (left + 15) / 16;
-              if (slab_is_cut(left, KE)) {
-                if (!mbar_poll(&fixed[s], (fixed_ph >> s) & 1u, wc, 24)) { ok = false; break; }
-                fixed_ph ^= 1u << s;
-              }
-            }
+          const int left = o.k - kb * KE;
+          // WGRAD: k-steps with rows of the group; else whole atoms (zeros behind K)
+          int steps = 4 * p.sub;
+          if (left < KE) steps = MODE == GMode::WGRAD ? (left + 15) / 16 : (left > KA ? 4 * p.sub : 4);
+          if (MODE == GMode::WGRAD && slab_is_cut(left, KE)) {
+            if (!mbar_poll(&fixed[s], (fixed_ph >> s) & 1u, wc, 24)) { ok = false; break; }
+            fixed_ph ^= 1u << s;
           }
           tc_fence_after();
-          const uint32_t aaddr = smem_u32(smem + static_cast<size_t>(s) * p.stage_bytes);
-          const uint32_t baddr = aaddr + kABytes;
+          const uint32_t abase = smem_u32(smem + static_cast<size_t>(s) * p.stage_bytes);
+          const uint32_t bbase = abase + p.sub * kABytes;
           for (int kk = 0; kk < steps; ++kk) {
             const uint32_t acc = (kb > 0 || kk > 0) ? 1u : 0u;
+            const uint32_t aaddr = abase + (kk >> 2) * kABytes, baddr = bbase + (kk >> 2) * b_bytes;
             uint64_t adesc, bdesc;
-            if constexpr (A_MN) adesc = sdesc_sw128(aaddr + kk * 16 * kSlabBytes, kBoxBytes, 1024);
-            else adesc = sdesc_sw128(aaddr + kk * 32, 16, 1024);
-            if constexpr (B_MN) bdesc = sdesc_sw128(baddr + kk * 16 * kSlabBytes, kBoxBytes, 1024);
-            else bdesc = sdesc_sw128(baddr + kk * 32, 16, 1024);
+            if constexpr (A_MN) adesc = sdesc_sw128(aaddr + (kk & 3) * 16 * kSlabBytes, kBoxBytes, 1024);
+            else adesc = sdesc_sw128(aaddr + (kk & 3) * 32, 16, 1024);
+            if constexpr (B_MN) bdesc = sdesc_sw128(baddr + (kk & 3) * 16 * kSlabBytes, kBoxBytes, 1024);
+            else bdesc = sdesc_sw128(baddr + (kk & 3) * 32, 16, 1024);
             if constexpr (KIND == Kind::F16) umma_f16(d_tmem, adesc, bdesc, idesc, acc);
             else umma_f8f6f4(d_tmem, adesc, bdesc, idesc, acc);
           }
@@ -497,10 +506,13 @@ __global__ void __launch_bounds__(kGroupedThreads, 1)
       if (!mbar_wait_warp(&tailfull[s], (cut_ph >> s) & 1u, wc, 26)) break;
       cut_ph ^= 1u << s;
       const uint32_t base = smem_u32(smem + static_cast<size_t>(s) * p.stage_bytes);
-      const int nz = ((left + 15) & ~15) - left;  // 1..15 rows of 128 bytes in each box
+      const int j = left / KA, at = left - j * KA;  // atom and row of the first row behind the end
+      const uint32_t a0 = base + j * kABytes, b0 = base + p.sub * kABytes + j * b_bytes;
+      const int nz = ((left + 15) & ~15) - left;    // 1..15 rows of 128 bytes in each box
       for (int i = lane; i < (2 + p.W / 64) * nz * 8; i += 32) {
         const int box = i / (nz * 8), rest = i - box * nz * 8;
-        st_shared_v4(base + box * kBoxBytes + (left + rest / 8) * kSlabBytes + (rest & 7) * 16, 0, 0, 0, 0);
+        st_shared_v4((box < 2 ? a0 + box * kBoxBytes : b0 + (box - 2) * kBoxBytes) + (at + rest / 8) * kSlabBytes +
+                         (rest & 7) * 16, 0, 0, 0, 0);
       }
       fence_proxy_async_smem();
       __syncwarp();
