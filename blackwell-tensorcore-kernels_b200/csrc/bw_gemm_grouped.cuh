@@ -138,6 +138,7 @@ __device__ __forceinline__ void grouped_scan(int groups, int tm, int per_row, in
 // group; WGRAD: of m), and the summed extent.
 struct GTile {
   int g, row0, rows, col0, kbase, k;
+  bool b_once;  // no other tile reads this one's columns of B
 };
 
 template <GMode MODE, int TM>
@@ -167,6 +168,7 @@ struct GWalk {
       o.rows = min(TM, m - o.row0);
       o.kbase = bounds[g];
       o.k = bounds[g + 1] - o.kbase;
+      o.b_once = true;
     } else {
       while (t >= tiles[g + 1]) ++g;
       const int first = bounds[g], n = bounds[g + 1] - first;
@@ -175,6 +177,7 @@ struct GWalk {
       o.rows = min(TM, n - tm * TM);
       o.kbase = 0;
       o.k = k;
+      o.b_once = n <= TM;
     }
     o.g = g;
     o.col0 = tn * W;
@@ -356,7 +359,10 @@ __global__ void __launch_bounds__(kGroupedThreads, 1)
   if (warp == 0) {
     // ---------------- TMA producer ----------------
     if (elect_one()) {
-      const uint64_t pol = l2_policy_evict_normal();
+      // A's rows are read by every tile of their group, B's columns (the weights) once where a group
+      // has one tile row: these then leave L2 first (64 matrices of 4096 x 2048 E4M3 and 1024 rows: 90.6 -> 84.8 us;
+      // for groups of more rows it costs 3%). WGRAD: Y's, which measured the same or 5-10% faster.
+      const uint64_t pol = l2_policy_evict_last(), pol_once = l2_policy_evict_first(), pol_more = l2_policy_evict_normal();
       int s = 0;
       uint32_t ph = 0;
       long long issued = 0;
@@ -365,6 +371,7 @@ __global__ void __launch_bounds__(kGroupedThreads, 1)
       for (int t = blockIdx.x; t < num_tiles && ok; t += gridDim.x) {
         const GTile o = walk.at(t);
         const int nk = (o.k + KE - 1) / KE;
+        const uint64_t pol_b = o.b_once ? pol_once : pol_more;
         for (int kb = 0; kb < nk; ++kb) {
           if (!mbar_poll(&empty[s], ph ^ 1, wc, 21)) { ok = false; break; }
           uint8_t* sA = smem + static_cast<size_t>(s) * p.stage_bytes;
@@ -389,7 +396,7 @@ __global__ void __launch_bounds__(kGroupedThreads, 1)
               tma_load_2d(&tmA, bar, sA + a * kABytes, o.row0, y, pol);
               tma_load_2d(&tmA, bar, sA + a * kABytes + kBoxBytes, o.row0 + 64, y, pol);
               for (int j = 0; j < p.W / 64; ++j)
-                tma_load_2d(&tmB, bar, sB + a * b_bytes + j * kBoxBytes, o.col0 + 64 * j, y, pol);
+                tma_load_2d(&tmB, bar, sB + a * b_bytes + j * kBoxBytes, o.col0 + 64 * j, y, pol_b);
             }
           } else {
             mbar_arrive_expect_tx(&full[s], atoms * (a_load_bytes(o.rows) + b_bytes));
@@ -403,9 +410,9 @@ __global__ void __launch_bounds__(kGroupedThreads, 1)
               }
               if constexpr (B_MN) {
                 for (int j = 0; j < p.W / 64; ++j)
-                  tma_load_3d(&tmB, &full[s], sB + a * b_bytes + j * kBoxBytes, o.col0 + 64 * j, x, o.g, pol);
+                  tma_load_3d(&tmB, &full[s], sB + a * b_bytes + j * kBoxBytes, o.col0 + 64 * j, x, o.g, pol_b);
               } else {
-                tma_load_3d(&tmB, &full[s], sB + a * b_bytes, x, o.col0, o.g, pol);
+                tma_load_3d(&tmB, &full[s], sB + a * b_bytes, x, o.col0, o.g, pol_b);
               }
             }
           }
@@ -645,7 +652,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGroupedThreads, 1)
         const int valid = min(128, o.rows - half);  // ROWS: this CTA's rows of the tile (may be <= 0)
         const uint32_t a_bytes = a_load_bytes(min(128, o.rows)) + (o.rows > 128 ? a_load_bytes(o.rows - 128) : 0);
         for (int kb = 0; kb < nk; ++kb) {
-          if (!mbar_poll(&empty[s], ph ^ 1, wc, 31)) { ok = false; break; }
+          if (!mbar_poll(&empty[s], ph ^ 1, wc, 61)) { ok = false; break; }
           uint8_t* sA = smem + s * kPairStageBytes;
           uint8_t* sB = sA + kPairSub * kPairAtom;
           uint32_t bar = full_leader + s * 8;
@@ -717,17 +724,17 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGroupedThreads, 1)
         const int b = local & 1;
         const uint32_t aph = (local >> 1) & 1;
         ++local;
-        if (!mbar_poll(&accempty[b], aph ^ 1, wc, 32)) { ok = false; break; }
+        if (!mbar_poll(&accempty[b], aph ^ 1, wc, 62)) { ok = false; break; }
         tc_fence_after();
         const uint32_t d_tmem = tmem_base + b * 256;
         for (int kb = 0; kb < nk; ++kb) {
-          if (!mbar_poll(&full[s], ph, wc, 33)) { ok = false; break; }
+          if (!mbar_poll(&full[s], ph, wc, 63)) { ok = false; break; }
           const int left = o.k - kb * KE;
           // WGRAD: k-steps with rows of the group; else whole atoms (zeros behind K)
           int steps = 4 * kPairSub;
           if (left < KE) steps = MODE == GMode::WGRAD ? (left + 15) / 16 : (left > KA ? 8 : 4);
           if (MODE == GMode::WGRAD && slab_is_cut(left, KE)) {
-            if (!mbar_wait_cluster(&fixed[s], (fixed_ph >> s) & 1u, wc, 34)) { ok = false; break; }
+            if (!mbar_wait_cluster(&fixed[s], (fixed_ph >> s) & 1u, wc, 64)) { ok = false; break; }
             fixed_ph ^= 1u << s;
           }
           tc_fence_after();
@@ -777,7 +784,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGroupedThreads, 1)
       const int b = local & 1;
       const uint32_t aph = (local >> 1) & 1;
       ++local;
-      if (!mbar_wait_warp(&accfull[b], aph, wc, 35)) break;
+      if (!mbar_wait_warp(&accfull[b], aph, wc, 65)) break;
       tc_fence_after();
       grouped_epilogue<MODE, OUT>(p, o, tmem_base + (static_cast<uint32_t>(q * 32) << 16) + b * 256, half + q * 32, lane,
                                   stage, [&] {
@@ -798,7 +805,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGroupedThreads, 1)
       issue += nk;
       if (nk == 0 || !slab_is_cut(left, KE)) continue;
       const int s = static_cast<int>((issue - 1) % S);
-      if (!mbar_wait_warp(&tailfull[s], (cut_ph >> s) & 1u, wc, 36)) break;
+      if (!mbar_wait_warp(&tailfull[s], (cut_ph >> s) & 1u, wc, 66)) break;
       cut_ph ^= 1u << s;
       const int j = left / KA, at = left - j * KA;  // atom and row of the first row behind the end
       const uint32_t base = smem_u32(smem + s * kPairStageBytes) + j * kPairAtom;

@@ -25,7 +25,8 @@ def _mul(p, **kw):
 
 @pytest.mark.parametrize("bad", [dict(dtype=bwgemm.DTYPE_F32), dict(dtype=bwgemm.DTYPE_MXFP4), dict(dtype=-1),
                                  dict(dtype=FP8), dict(out=2), dict(rows=-1), dict(N=-1), dict(K=-1), dict(groups=0),
-                                 dict(groups=-3), dict(groups=1025), dict(off=None), dict(A=None), dict(B=None),
+                                 dict(groups=-3), dict(groups=1025), dict(off=None), dict(rows=2 ** 31 - 1),
+                                 dict(N=2 ** 31 - 8, ldc=2 ** 31), dict(K=2 ** 31 - 16, lda=2 ** 31), dict(A=None), dict(B=None),
                                  dict(C=None), dict(lda=15), dict(lda=8), dict(lda=20), dict(ldc=15), dict(N=12),
                                  dict(t=1, K=12), dict(t=1, dtype=FP8, K=8, lda=16), dict(t=1, dtype=FP8, lda=24)])
 def test_refuses(p, bad):

@@ -220,6 +220,54 @@ def test_exact_integers(cuda_dev):
     assert torch.equal(C.double(), want)
 
 
+@pytest.mark.parametrize("which", ["rows", "groups", "both"])
+def test_scales_of_16_bit_products(cuda_dev, which):
+    """Row and group scales are taken with every operand type, each alone too."""
+    import torch
+
+    offsets = [0, 40, 40, 300]
+    off = torch.tensor(offsets, dtype=torch.int32, device=cuda_dev)
+    a, b, _, _, ad, bd = _make(cuda_dev, "bfloat16", "kn", 3, 300, 264, 136)
+    rs = torch.rand(300, device=cuda_dev) + 0.5 if which != "groups" else None
+    gs = torch.rand(3, device=cuda_dev) + 0.5 if which != "rows" else None
+    C = bwgemm.gemm_grouped(a, b, off, row_scale=rs, group_scale=gs, out_dtype=F32)
+    want, mag = _product(ad, bd, "kn", offsets, rs, gs)
+    _close(C, want, mag, _steps("bf16", 136), F32)
+
+
+def test_dependent_calls_in_a_row(cuda_dev):
+    """Each call reads what the one before it wrote, and writes what that one read, without a pause:
+    the same bits as with a synchronisation after every call."""
+    import torch
+
+    offsets = [0, 130, 131, 400, 700]
+    off = torch.tensor(offsets, dtype=torch.int32, device=cuda_dev)
+    g = torch.Generator(device=cuda_dev).manual_seed(2)
+    a0 = torch.randn(700, 512, device=cuda_dev, generator=g).bfloat16()
+    b = (torch.randn(4, 512, 512, device=cuda_dev, generator=g) * 512 ** -0.5).bfloat16()
+    w = torch.ones(512, device=cuda_dev).bfloat16()
+
+    def chain(pause):
+        one, two = a0.clone(), torch.empty_like(a0)
+        grads = torch.zeros(4, 512, 512, device=cuda_dev)
+        for i in range(20):
+            for x, y in ((one, two), (two, one)):
+                bwgemm.gemm_grouped(x, b, off, y, b_transposed=bool(i % 2))
+                pause()
+                bwgemm.gemm_grouped_wgrad(x, y, off, grads)
+                pause()
+                bwgemm.rmsnorm(y, w, y=y)
+                pause()
+                off.copy_(torch.roll(off, 0))
+        return one, two, grads
+
+    want = chain(torch.cuda.synchronize)
+    for _ in range(3):
+        got = chain(lambda: None)
+        torch.cuda.synchronize()
+        assert all(torch.equal(p, q) for p, q in zip(got, want))
+
+
 def test_many_groups(cuda_dev):
     """1024 groups, most of them empty or of one row."""
     import torch
