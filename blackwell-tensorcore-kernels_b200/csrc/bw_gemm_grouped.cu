@@ -123,17 +123,7 @@ int launch(const Operands& o, int dtype, GroupedParams p, cudaStream_t s, const 
   const int cap = env_int("BW_MAX_CTAS", 0);
   if (cap > 0 && room > cap / (pair ? 2 : 1)) room = cap / (pair ? 2 : 1) > 0 ? cap / (pair ? 2 : 1) : 1;
   const int n = static_cast<int>(most < room ? most : room);
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(pair ? 2 * n : n);
-  cfg.blockDim = dim3(kGroupedThreads);
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = s;
-  cudaLaunchAttribute attr = {};
-  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;  // see grid_dependency_wait
-  attr.val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = &attr;
-  cfg.numAttrs = 1;
-  BW_CUDA(cudaLaunchKernelEx(&cfg, pair ? two : one, ta, ta16, tb, p));
+  BW_CUDA(launch_dependent(pair ? two : one, dim3(pair ? 2 * n : n), kGroupedThreads, smem, s, ta, ta16, tb, p));
   return BW_OK;
 }
 

@@ -92,14 +92,6 @@ __device__ __forceinline__ void mbar_drain(uint64_t* bar, uint32_t parity, uint6
   }
 }
 
-// Programmatic dependent launch: a grid may start while the one before it in the stream ends, and
-// waits here for that one's end (and its writes) before it touches global memory; it lets the next
-// grid start the same way. Barriers, Tensor Memory and descriptors are set up in the meantime.
-__device__ __forceinline__ void grid_dependency_wait() {
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  asm volatile("griddepcontrol.wait;" ::: "memory");
-}
-
 // bounds[g] = first row of group g (bounds[groups] = end of the last), clamped and made
 // non-decreasing; tiles[g] = output tiles of the groups before g, `per_row` of them per tm rows.
 // All threads fetch the offsets (one trip to memory); warp 2 scans them.

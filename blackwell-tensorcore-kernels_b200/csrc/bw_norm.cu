@@ -23,6 +23,7 @@
 #include <cmath>
 #include <type_traits>
 
+#include "bw_ptx.cuh"
 #include "bw_runtime.cuh"
 
 namespace bw {
@@ -331,6 +332,7 @@ constexpr int kThreadBytes = NV * (sizeof(T) * VE < 4 ? 4 : sizeof(T) * VE);
 template <typename T, typename WT, bool Q8, int VE, int NV, bool SHIFT>
 __global__ void __launch_bounds__(512) k_rmsnorm(const NormParams p, int tpr) {
   constexpr bool kKeep = kThreadBytes<T, VE, NV> <= 64;
+  grid_dependency_wait();
   __shared__ SumMax sm[2][32];
   const int per_block = blockDim.x / tpr;
   const int t = threadIdx.x % tpr;
@@ -402,6 +404,7 @@ __global__ void __launch_bounds__(512) k_rmsnorm(const NormParams p, int tpr) {
 template <typename T, typename WT, bool Q8, int VE>
 __global__ void __launch_bounds__(1024) k_rmsnorm_wide(const NormParams p) {
   __shared__ SumMax sm[32];
+  grid_dependency_wait();
   const long long row = blockIdx.x;
   const T* x = static_cast<const T*>(p.x) + row * p.ldx;
   const T* r = p.res ? static_cast<const T*>(p.res) + row * p.ldr : nullptr;
@@ -461,6 +464,7 @@ struct NormGradParams {
 template <typename T, typename WT, int VE, int NV, bool SHIFT>
 __global__ void __launch_bounds__(512) k_rmsnorm_grad(const NormGradParams p, int tpr) {
   constexpr bool kKeep = kThreadBytes<T, VE, NV> <= 32;
+  grid_dependency_wait();
   __shared__ SumMax sm[2][32];
   extern __shared__ float cols_sum[];  // tpr <= 32: [group of the block][cols]
   const int per_block = blockDim.x / tpr, mine = threadIdx.x / tpr;
@@ -575,6 +579,7 @@ __global__ void __launch_bounds__(512) k_rmsnorm_grad(const NormGradParams p, in
 template <typename T, typename WT>
 __global__ void __launch_bounds__(1024) k_rmsnorm_grad_wide(const NormGradParams p) {
   __shared__ SumMax sm[32];
+  grid_dependency_wait();
   const long long row = blockIdx.x;
   const T* dy = static_cast<const T*>(p.dy) + row * p.lddy;
   const T* h = static_cast<const T*>(p.h) + row * p.ldh;
@@ -592,6 +597,7 @@ __global__ void __launch_bounds__(1024) k_rmsnorm_grad_wide(const NormGradParams
 }
 template <typename T>
 __global__ void __launch_bounds__(256) k_rmsnorm_dw_wide(const NormGradParams p) {
+  grid_dependency_wait();
   const long long c = blockIdx.x * 256LL + threadIdx.x;
   if (c >= p.cols) return;
   for (int slab = blockIdx.y; slab < p.slabs; slab += gridDim.y) {
@@ -607,6 +613,7 @@ __global__ void __launch_bounds__(256) k_rmsnorm_dw_wide(const NormGradParams p)
 __global__ void __launch_bounds__(1024) k_sum_slabs(const float* __restrict__ partial, float* __restrict__ dw,
                                                     int slabs, int cols) {
   __shared__ float sm[32][33];
+  grid_dependency_wait();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const long long c = blockIdx.x * 32LL + lane;
   float s = 0.f;
@@ -690,8 +697,7 @@ int launch_rows(Kernel kern, const NormParams& p, const Shape& sh, bool shift, c
   long long cap = static_cast<long long>(d.sms) * per_sm;
   if (shift) cap = cap / 8 * 8;  // a stride of whole phases
   if (grid > cap) grid = cap;
-  kern<<<static_cast<unsigned>(grid), sh.block, 0, s>>>(p, sh.tpr);
-  BW_CUDA(cudaGetLastError());
+  BW_CUDA(launch_dependent(kern, dim3(static_cast<unsigned>(grid)), sh.block, 0, s, p, sh.tpr));
   return BW_OK;
 }
 
@@ -702,8 +708,7 @@ int launch_norm(const NormParams& p, cudaStream_t s, const DeviceState& d) {
   const Shape sh = row_shape(p.rows, nvec, 4, kMaxNv, SHIFT ? 16 : 1);
   if (sh.nv == 0) {
     constexpr int WVE = SHIFT ? 1 : VE;
-    k_rmsnorm_wide<T, WT, Q8, WVE><<<static_cast<unsigned>(p.rows), 1024, 0, s>>>(p);
-    BW_CUDA(cudaGetLastError());
+    BW_CUDA(launch_dependent(k_rmsnorm_wide<T, WT, Q8, WVE>, dim3(static_cast<unsigned>(p.rows)), 1024, 0, s, p));
     return BW_OK;
   }
   switch (sh.nv) {
@@ -822,29 +827,28 @@ int launch_grad(NormGradParams p, float* dw, cudaStream_t s) {
   const Shape sh = row_shape(p.rows, nvec, sizeof(T) == 4 && p.rows >= 2048 ? 4 : 2, kMaxNv, SHIFT ? 16 : 1);
   if (sh.nv == 0) {
     // the weight gradient first: dx may be written over dy or h
-    k_rmsnorm_dw_wide<T><<<dim3(static_cast<unsigned>((p.cols + 255LL) / 256), p.slabs), 256, 0, s>>>(p);
-    BW_CUDA(cudaGetLastError());
-    k_rmsnorm_grad_wide<T, WT><<<static_cast<unsigned>(p.rows), 1024, 0, s>>>(p);
+    BW_CUDA(launch_dependent(k_rmsnorm_dw_wide<T>, dim3(static_cast<unsigned>((p.cols + 255LL) / 256), p.slabs), 256, 0, s, p));
+    BW_CUDA(launch_dependent(k_rmsnorm_grad_wide<T, WT>, dim3(static_cast<unsigned>(p.rows)), 1024, 0, s, p));
   } else {
     const long long groups = (p.rows + sh.groups - 1) / sh.groups;
     if (groups <= p.slabs) p.slabs = static_cast<int>(groups);  // a row each
     else if (SHIFT && sh.groups < 8) p.slabs = p.slabs / 8 * 8;  // a stride of whole phases
     const size_t smem = sh.tpr > 32 ? 0 : static_cast<size_t>(sh.groups) * p.cols * sizeof(float);
+    auto go = [&](auto kern) { return launch_dependent(kern, dim3(p.slabs), sh.block, smem, s, p, sh.tpr); };
     switch (sh.nv) {
-      case 1: k_rmsnorm_grad<T, WT, VE, 1, SHIFT><<<p.slabs, sh.block, smem, s>>>(p, sh.tpr); break;
-      case 2: k_rmsnorm_grad<T, WT, VE, 2, SHIFT><<<p.slabs, sh.block, smem, s>>>(p, sh.tpr); break;
-      case 4: k_rmsnorm_grad<T, WT, VE, 4, SHIFT><<<p.slabs, sh.block, smem, s>>>(p, sh.tpr); break;
+      case 1: BW_CUDA(go(k_rmsnorm_grad<T, WT, VE, 1, SHIFT>)); break;
+      case 2: BW_CUDA(go(k_rmsnorm_grad<T, WT, VE, 2, SHIFT>)); break;
+      case 4: BW_CUDA(go(k_rmsnorm_grad<T, WT, VE, 4, SHIFT>)); break;
       case 8:
-        if constexpr (kMaxNv >= 8) k_rmsnorm_grad<T, WT, VE, 8, SHIFT><<<p.slabs, sh.block, smem, s>>>(p, sh.tpr);
+        if constexpr (kMaxNv >= 8) BW_CUDA(go(k_rmsnorm_grad<T, WT, VE, 8, SHIFT>));
         break;
       default:
-        if constexpr (kMaxNv >= 16) k_rmsnorm_grad<T, WT, VE, 16, SHIFT><<<p.slabs, sh.block, smem, s>>>(p, sh.tpr);
+        if constexpr (kMaxNv >= 16) BW_CUDA(go(k_rmsnorm_grad<T, WT, VE, 16, SHIFT>));
         break;
     }
   }
-  BW_CUDA(cudaGetLastError());
-  k_sum_slabs<<<static_cast<unsigned>((p.cols + 31LL) / 32), 1024, 0, s>>>(p.partial, dw, p.slabs, p.cols);
-  BW_CUDA(cudaGetLastError());
+  BW_CUDA(launch_dependent(k_sum_slabs, dim3(static_cast<unsigned>((p.cols + 31LL) / 32)), 1024, 0, s,
+                           static_cast<const float*>(p.partial), dw, p.slabs, p.cols));
   return BW_OK;
 }
 

@@ -431,3 +431,14 @@ __device__ __forceinline__ void bulk_load_cluster_bar(void* dst, const void* src
       : "memory");
 }
 }  // namespace bw
+
+namespace bw {
+// Programmatic dependent launch: a grid may start while the one before it in the stream ends, and
+// waits here for that one's end (and its writes) before it touches global memory; it lets the next
+// grid start the same way. What needs no global memory is set up in the meantime. Kernels that call
+// this are launched through launch_dependent (bw_runtime.cuh).
+__device__ __forceinline__ void grid_dependency_wait() {
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+}
+}  // namespace bw

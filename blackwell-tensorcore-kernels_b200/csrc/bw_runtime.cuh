@@ -86,6 +86,22 @@ int pair_clusters_resident(Kernel kern, int threads, int smem_bytes, const Devic
   return n;
 }
 
+// Launches a kernel that waits for the one before it by itself (grid_dependency_wait, bw_ptx.cuh).
+template <typename Kernel, typename... Args>
+cudaError_t launch_dependent(Kernel kern, dim3 grid, int block, size_t smem, cudaStream_t stream, const Args&... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(block);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr = {};
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kern, args...);
+}
+
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
 }  // namespace bw
