@@ -14,6 +14,7 @@ from __future__ import annotations
 
 import contextlib
 import ctypes
+import functools
 import os
 import re
 import subprocess
@@ -446,11 +447,17 @@ def rmsnorm_fp8(x, weight, residual=None, eps: float = 1e-6, q=None, row_scale=N
     return q, row_scale, h, rstd
 
 
+@functools.lru_cache(maxsize=256)
+def rmsnorm_backward_workspace(rows: int, cols: int) -> int:
+    """Bytes of workspace that rmsnorm_backward needs for these sizes."""
+    return int(lib().bw_rmsnorm_backward_workspace(rows, cols))
+
+
 def rmsnorm_backward(dy, h, weight, rstd, dresidual=None, dx=None, dweight=None, workspace=None, stream=None):
     """Gradient of rmsnorm from the h and rstd it returned: (dx, dweight). dx is the gradient of x
     and of the residual alike, with dresidual (the gradient that reached h past the norm) added;
     dweight is float32. dx may be dy's, h's or dresidual's own tensor. `workspace`: uint8 tensor of
-    bw_rmsnorm_backward_workspace(rows, cols) bytes; one of the call's own where None."""
+    rmsnorm_backward_workspace(rows, cols) bytes; one of the call's own where None."""
     import torch
 
     code, wcode, dtype, shape, dev, ldh, lddr = _norm_operands(h, weight, dresidual)
@@ -467,7 +474,7 @@ def rmsnorm_backward(dy, h, weight, rstd, dresidual=None, dx=None, dweight=None,
         else:
             _flat("dweight", dweight, shape[1:], torch.float32, dev)
         if workspace is None:
-            nbytes = lib().bw_rmsnorm_backward_workspace(*shape)
+            nbytes = rmsnorm_backward_workspace(*shape)
             workspace = torch.empty_strided((nbytes,), (1,), dtype=torch.uint8, device=h.device)
         else:
             nbytes = workspace.numel()

@@ -94,9 +94,10 @@ __device__ __forceinline__ void mbar_drain(uint64_t* bar, uint32_t parity, uint6
 
 // bounds[g] = first row of group g (bounds[groups] = end of the last), clamped and made
 // non-decreasing; tiles[g] = output tiles of the groups before g, `per_row` of them per tm rows.
-// All threads fetch the offsets (one trip to memory); warp 2 scans them.
+// All threads fetch the offsets (one trip to memory, past L1: the kernel before may just have written
+// them); warp 2 scans them.
 __device__ __forceinline__ void grouped_fetch(const int* offsets, int groups, int rows, int* bounds) {
-  for (int g = threadIdx.x; g <= groups; g += kGroupedThreads) bounds[g] = min(max(__ldg(offsets + g), 0), rows);
+  for (int g = threadIdx.x; g <= groups; g += kGroupedThreads) bounds[g] = min(max(__ldcg(offsets + g), 0), rows);
 }
 __device__ __forceinline__ void grouped_scan(int groups, int tm, int per_row, int* bounds, int* tiles) {
   const int lane = threadIdx.x & 31;
@@ -201,8 +202,8 @@ __device__ __forceinline__ void grouped_epilogue(const GroupedParams& p, const G
   } else {
     row = t.row0 + first;
     if (t.k > 0) {
-      if (p.group_scale) alpha *= __ldg(p.group_scale + t.g);
-      if (p.row_scale && lane < nrows) alpha *= __ldg(p.row_scale + row + lane);
+      if (p.group_scale) alpha *= __ldcg(p.group_scale + t.g);
+      if (p.row_scale && lane < nrows) alpha *= __ldcg(p.row_scale + row + lane);
     }
   }
   const long long pitch = p.ldc * kElem;

@@ -458,7 +458,9 @@ struct NormGradParams {
 
 // Rows, columns and phases as in k_rmsnorm; each thread keeps the weight gradient of its own
 // columns in registers over all its rows. With g = dy w:
-//   dx = rstd g - h (rstd^3 / cols) sum(g h) + dresidual,   dw += (dy rstd) h
+//   dx = rstd (g - n m) + dresidual,   n = h rstd,   m = rstd sum(g h) / cols,   dw += (dy rstd) h
+// (one product more an element than rstd g - h rstd^3 sum / cols, whose cube leaves FP32 for rows of
+// 10^13 or 10^-13).
 // Where a thread holds up to 32 bytes of a row it keeps its weights and fetches the next row during this
 // one's reduction; else it reads the weights again and dresidual late.
 template <typename T, typename WT, int VE, int NV, bool SHIFT>
@@ -529,7 +531,7 @@ __global__ void __launch_bounds__(512) k_rmsnorm_grad(const NormGradParams p, in
     a = reduce_row(a, tpr, sm[half]);
     half ^= 1;
     if (live) {
-      const float coef = rstd * rstd * rstd * (a.sum * inv_cols);
+      const float m = rstd * (a.sum * inv_cols);
       if constexpr (!kKeep)
         if (drs) load_row(drs + row * p.lddr, c, dr);
 #pragma unroll
@@ -538,13 +540,13 @@ __global__ void __launch_bounds__(512) k_rmsnorm_grad(const NormGradParams p, in
         float o[VE];
 #pragma unroll
         for (int j = 0; j < VE; ++j) {
-          o[j] = elem<T>(dy.v[i], j) * elem<WT>(w[kKeep ? i : 0], j) * rstd - elem<T>(h.v[i], j) * coef;
+          o[j] = rstd * (elem<T>(dy.v[i], j) * elem<WT>(w[kKeep ? i : 0], j) - elem<T>(h.v[i], j) * rstd * m);
           if (drs) o[j] += elem<T>(dr.v[i], j);
         }
         dy.v[i] = from_floats<T, VE>(o);
       }
       if constexpr (SHIFT) {
-        dy.one = dy.one * w1 * rstd - h.one * coef;
+        dy.one = rstd * (dy.one * w1 - h.one * rstd * m);
         if (drs) dy.one += dr.one;
       }
       store_row(static_cast<T*>(p.dx) + row * p.lddx, c, dy);
@@ -588,9 +590,9 @@ __global__ void __launch_bounds__(1024) k_rmsnorm_grad_wide(const NormGradParams
   SumMax a{0.f, 0.f};
   for (long long c = threadIdx.x; c < p.cols; c += 1024) a.sum = fmaf(to_f32(dy[c]) * to_f32(w[c]), to_f32(h[c]), a.sum);
   a = reduce_row(a, 1024, sm);
-  const float coef = rstd * rstd * rstd * (a.sum / static_cast<float>(p.cols));
+  const float m = rstd * (a.sum / static_cast<float>(p.cols));
   for (long long c = threadIdx.x; c < p.cols; c += 1024) {
-    float g = to_f32(dy[c]) * to_f32(w[c]) * rstd - to_f32(h[c]) * coef;
+    float g = rstd * (to_f32(dy[c]) * to_f32(w[c]) - to_f32(h[c]) * rstd * m);
     if (p.dres) g += to_f32(static_cast<const T*>(p.dres)[row * p.lddr + c]);
     static_cast<T*>(p.dx)[row * p.lddx + c] = from_f32<T>(g);
   }
@@ -610,15 +612,14 @@ __global__ void __launch_bounds__(256) k_rmsnorm_dw_wide(const NormGradParams p)
 }
 
 // dw[c] = sum over slabs in a fixed order: 32 columns a block, 32 warps over the slabs.
-__global__ void __launch_bounds__(1024) k_sum_slabs(const float* __restrict__ partial, float* __restrict__ dw,
-                                                    int slabs, int cols) {
+__global__ void __launch_bounds__(1024) k_sum_slabs(const float* partial, float* dw, int slabs, int cols) {
   __shared__ float sm[32][33];
   grid_dependency_wait();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const long long c = blockIdx.x * 32LL + lane;
   float s = 0.f;
   if (c < cols)
-    for (int i = warp; i < slabs; i += 32) s += partial[static_cast<long long>(i) * cols + c];
+    for (int i = warp; i < slabs; i += 32) s += __ldcg(partial + static_cast<long long>(i) * cols + c);
   sm[warp][lane] = s;
   __syncthreads();
   s = sm[lane][warp];  // column blockIdx.x * 32 + warp, partial sum `lane`
@@ -684,20 +685,20 @@ Access row_access(const RowsOf (&t)[N], int ve, long long cols, int* phase) {
 
 // As many blocks as are resident at once (16384 x 8192 BF16: 141 us; with one more a SM 143 us, and with
 // a few left over twice as long), each with its share of the rows.
-template <typename Kernel>
-int launch_rows(Kernel kern, const NormParams& p, const Shape& sh, bool shift, cudaStream_t s, const DeviceState& d) {
+template <auto KERN, bool SHIFT>
+int launch_rows(const NormParams& p, const Shape& sh, cudaStream_t s, const DeviceState& d) {
   static std::atomic<int> resident[kMaxThreads / 32 + 1] = {};  // by block size, of this kernel; 0: not asked yet
   std::atomic<int>& known = resident[sh.block / 32];
   int per_sm = known.load(std::memory_order_relaxed);
   if (per_sm == 0) {
-    BW_CUDA(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kern, sh.block, 0));
+    BW_CUDA(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, KERN, sh.block, 0));
     known.store(per_sm, std::memory_order_relaxed);
   }
   long long grid = (p.rows + sh.groups - 1) / sh.groups;
   long long cap = static_cast<long long>(d.sms) * per_sm;
-  if (shift) cap = cap / 8 * 8;  // a stride of whole phases
+  if (SHIFT) cap = cap / 8 * 8;  // a stride of whole phases
   if (grid > cap) grid = cap;
-  BW_CUDA(launch_dependent(kern, dim3(static_cast<unsigned>(grid)), sh.block, 0, s, p, sh.tpr));
+  BW_CUDA(launch_dependent(KERN, dim3(static_cast<unsigned>(grid)), sh.block, 0, s, p, sh.tpr));
   return BW_OK;
 }
 
@@ -712,14 +713,14 @@ int launch_norm(const NormParams& p, cudaStream_t s, const DeviceState& d) {
     return BW_OK;
   }
   switch (sh.nv) {
-    case 1: return launch_rows(k_rmsnorm<T, WT, Q8, VE, 1, SHIFT>, p, sh, SHIFT, s, d);
-    case 2: return launch_rows(k_rmsnorm<T, WT, Q8, VE, 2, SHIFT>, p, sh, SHIFT, s, d);
-    case 4: return launch_rows(k_rmsnorm<T, WT, Q8, VE, 4, SHIFT>, p, sh, SHIFT, s, d);
+    case 1: return launch_rows<k_rmsnorm<T, WT, Q8, VE, 1, SHIFT>, SHIFT>(p, sh, s, d);
+    case 2: return launch_rows<k_rmsnorm<T, WT, Q8, VE, 2, SHIFT>, SHIFT>(p, sh, s, d);
+    case 4: return launch_rows<k_rmsnorm<T, WT, Q8, VE, 4, SHIFT>, SHIFT>(p, sh, s, d);
     case 8:
-      if constexpr (kMaxNv >= 8) return launch_rows(k_rmsnorm<T, WT, Q8, VE, 8, SHIFT>, p, sh, SHIFT, s, d);
+      if constexpr (kMaxNv >= 8) return launch_rows<k_rmsnorm<T, WT, Q8, VE, 8, SHIFT>, SHIFT>(p, sh, s, d);
       [[fallthrough]];
     default:
-      if constexpr (kMaxNv >= 16) return launch_rows(k_rmsnorm<T, WT, Q8, VE, 16, SHIFT>, p, sh, SHIFT, s, d);
+      if constexpr (kMaxNv >= 16) return launch_rows<k_rmsnorm<T, WT, Q8, VE, 16, SHIFT>, SHIFT>(p, sh, s, d);
       return BW_OK;  // row_shape gives no more than kMaxNv
   }
 }

@@ -164,7 +164,8 @@ size_t bw_sf_offset(int row, int kblock, int K);
  * h and rstd may be NULL (not wanted). ld*: row pitches in elements, at least cols. Any alignment
  * to whole elements; 16-byte aligned rows run faster. y and h may be x's or the residual's own
  * buffer (same type, same pitch); other overlap is not allowed. Sums are FP32: a row whose squares
- * sum to more than FP32 holds gets rstd = 0, one with a NaN gets NaN (codes 0x7f, scale 1). */
+ * sum to more than FP32 holds gets rstd = 0, one with a NaN, or of zeros with eps = 0, gets NaN (codes
+ * 0x7f, scale 1). */
 int bw_rmsnorm(const void* x, long long ldx, const void* residual, long long ldr, const void* weight, int dtype,
                int weight_dtype, float eps, void* y, long long ldy, void* h, long long ldh, float* rstd, int rows,
                int cols, void* stream);

@@ -425,6 +425,45 @@ def test_graph_replays_with_new_sizes(cuda_dev):
             _check_wgrad(x, y, new, D, F32)
 
 
+def test_capture_with_fork_and_join(cuda_dev):
+    """Captured behind a copy, a memset and another stream's kernels: full dependencies are kept."""
+    import torch
+
+    a, b, rs, gs, _, _ = _make(cuda_dev, "fp8", "nk", 4, 500, 264, 256)
+    A, off = torch.zeros_like(a.contiguous()), torch.zeros(5, dtype=torch.int32, device=cuda_dev)
+    true = torch.tensor([0, 100, 100, 330, 500], dtype=torch.int32, device=cuda_dev)
+    y = torch.randn(500, 72, device=cuda_dev).bfloat16()
+    side = torch.cuda.Stream(cuda_dev)
+
+    def work():
+        main = torch.cuda.current_stream()
+        side.wait_stream(main)
+        A.copy_(a)
+        with torch.cuda.stream(side):
+            off.zero_()
+            off.add_(true)
+        main.wait_stream(side)
+        C = bwgemm.gemm_grouped(A, b, off, b_transposed=True, row_scale=rs, group_scale=gs)
+        side.wait_stream(main)
+        with torch.cuda.stream(side):
+            D = bwgemm.gemm_grouped_wgrad(C, y, off)
+        E = C * 2
+        main.wait_stream(side)
+        return C, D, E
+
+    want = work()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = work()
+    for _ in range(4):
+        A.zero_(), off.fill_(7)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert bwgemm.device_status() == 0
+        assert all(torch.equal(p, q) for p, q in zip(want, got))
+
+
 def test_repeatable(cuda_dev):
     """The same call twice gives the same bits."""
     import torch

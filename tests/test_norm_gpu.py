@@ -258,6 +258,75 @@ def test_backward_against_differences(cuda_dev):
         assert abs(float(num) - float(dw[j])) <= 1e-5 * (1 + abs(float(num)))
 
 
+@pytest.mark.parametrize("size", [1e-15, 1e-6, 1e6, 1e15])
+def test_magnitudes(cuda_dev, size):
+    """Rows of very small and very large values: no intermediate power of rstd leaves FP32."""
+    import torch
+
+    for cols in (64, 1001, 20000):
+        x, r, w = _inputs(cuda_dev, torch.float32, 3, cols, True)
+        x, r = x * size, r * size
+        y, h, rstd = bwgemm.rmsnorm(x, w, residual=r, eps=0.0)
+        _check_forward(x, r, w, y, h, rstd, eps=0.0)
+        q, s, h, rstd = bwgemm.rmsnorm_fp8(x, w, residual=r, eps=0.0)
+        _check_fp8(x, r, w, q, s, h, rstd, eps=0.0)
+        g = torch.Generator(device=cuda_dev).manual_seed(8)
+        dy = torch.randn(3, cols, device=cuda_dev, generator=g)
+        dx, dw = bwgemm.rmsnorm_backward(dy, h, w, rstd)
+        _check_backward(dy, h, w, rstd, None, dx, dw)
+
+
+def test_zero_row_without_eps(cuda_dev):
+    """0 / 0: NaN in the row, not in its neighbours."""
+    import torch
+
+    x = torch.ones(3, 40, device=cuda_dev)
+    x[1] = 0
+    w = torch.ones(40, device=cuda_dev)
+    y, _, _ = bwgemm.rmsnorm(x, w, eps=0.0)
+    q, s, _, _ = bwgemm.rmsnorm_fp8(x, w, eps=0.0)
+    assert bool(y[1].isnan().all()) and bool((q[1] & 0x7F == 0x7F).all()) and float(s[1]) == 1.0
+    assert bool((y[[0, 2]] == 1).all()) and bool((s[[0, 2]] == torch.tensor(1.0) / 448).all())
+
+
+def test_capture_with_fork_and_join(cuda_dev):
+    """Captured behind a copy, a memset and another stream's kernels: full dependencies are kept."""
+    import torch
+
+    w = torch.ones(512, device=cuda_dev, dtype=torch.bfloat16)
+    src, res, dy = (torch.randn(300, 512, device=cuda_dev).bfloat16() for _ in range(3))
+    x, r, g = torch.zeros_like(src), torch.zeros_like(src), torch.zeros_like(src)
+    side = torch.cuda.Stream(cuda_dev)
+
+    def work():
+        main = torch.cuda.current_stream()
+        side.wait_stream(main)
+        x.copy_(src)
+        with torch.cuda.stream(side):
+            r.zero_()
+            r.add_(res)
+            g.copy_(dy)
+        main.wait_stream(side)
+        y, h, rstd = bwgemm.rmsnorm(x, w, residual=r)
+        side.wait_stream(main)
+        with torch.cuda.stream(side):
+            dx, dw = bwgemm.rmsnorm_backward(g, h, w, rstd)
+        q, s, _, _ = bwgemm.rmsnorm_fp8(y, w)
+        main.wait_stream(side)
+        return y, dx, dw, q, s
+
+    want = work()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = work()
+    for _ in range(4):
+        x.zero_(), r.fill_(5), g.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(want, got))
+
+
 def test_empty(cuda_dev):
     import torch
 
