@@ -13,8 +13,8 @@
 // reduction and its output. max |y| needs no second reduction: y_j = (h_j w_j) rstd and rounding is
 // monotonic, so max |y| = max |h w| * rstd exactly, and both sums travel through one reduction.
 // Statistics and sums are FP32. Measured, 16384 x 8192 BF16 with residual: to E4M3 140 us (6.7 TB/s of
-// the 7 bytes an element), gradient 178 us (6.0 TB/s of 8 bytes); 131072 x 128 BF16 to BF16 11.0 us
-// (6.2 TB/s); 8192 x 4095 to E4M3, rows at every alignment, 50 us; one row of 8192 3 us.
+// the 7 bytes an element), gradient 175 us (6.1 TB/s of 8 bytes); 131072 x 128 BF16 to BF16 10.5 us
+// (6.4 TB/s); 8192 x 4095 to E4M3, rows at every alignment, 50 us; one row of 8192 2.8 us.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_fp8.h>
@@ -457,7 +457,8 @@ struct NormGradParams {
 };
 
 // Rows, columns and phases as in k_rmsnorm; each thread keeps the weight gradient of its own
-// columns in registers over all its rows. With g = dy w:
+// columns in registers over all its rows, and stores it four columns at a time (64 x 8192 BF16 10.6 us one
+// by one, 6.6 us so; through shared memory, for columns behind a boundary, measured slower). With g = dy w:
 //   dx = rstd (g - n m) + dresidual,   n = h rstd,   m = rstd sum(g h) / cols,   dw += (dy rstd) h
 // (one product more an element than rstd g - h rstd^3 sum / cols, whose cube leaves FP32 for rows of
 // 10^13 or 10^-13).
@@ -563,8 +564,15 @@ __global__ void __launch_bounds__(512) k_rmsnorm_grad(const NormGradParams p, in
 #pragma unroll
   for (int i = 0; i < NV; ++i)
     if (c.has(i)) {
+      float* at = mine_out + c.col(i);
+      if (VE % 4 == 0 && (reinterpret_cast<uintptr_t>(at) & 15) == 0) {
 #pragma unroll
-      for (int j = 0; j < VE; ++j) mine_out[c.col(i) + j] = dw[i][j];
+        for (int j = 0; j + 3 < VE; j += 4)
+          *reinterpret_cast<float4*>(at + j) = make_float4(dw[i][j], dw[i][j + 1], dw[i][j + 2], dw[i][j + 3]);
+      } else {
+#pragma unroll
+        for (int j = 0; j < VE; ++j) at[j] = dw[i][j];
+      }
     }
   if (SHIFT && c.single >= 0) mine_out[c.single] = dw1;
   if (tpr > 32) return;
@@ -640,12 +648,14 @@ struct Shape {
   long long groups;  // a block
 };
 
-// Threads a row (at least min_tpr) and vectors a thread (1, 2, 4, ... up to max_nv). Few rows: a vector a thread (each load
-// waits once). Many: `want` vectors, so that a block is small and each thread has more loads in flight;
-// fewer where a warp's granularity would leave over an eighth more of them idle.
+// Threads a row (at least min_tpr) and vectors a thread (1, 2, 4, ... up to max_nv): `want` vectors, so that a
+// block is small and each thread has more loads in flight, but one where that still gives every
+// resident thread (512 an SM) at most one (BF16 to E4M3 with one / four: 150 x 512 2.3 / 3.0 us, 150 x 2048
+// 2.6 / 2.8, 300 x 2048 3.2 / 3.2, 150 x 8192 4.6 / 3.8, 1200 x 8192 16.2 / 12.9); fewer also where a warp's
+// granularity would leave over an eighth more of them idle.
 constexpr int kMaxThreads = 512;
 Shape row_shape(long long rows, long long nvec, int want, int max_nv, int min_tpr) {
-  if (rows < 512) want = 1;
+  if (rows * nvec <= 148LL * 512) want = 1;
   int nv = want;
   while (nv <= max_nv && nvec > static_cast<long long>(nv) * kMaxThreads) nv *= 2;
   if (nv > max_nv) return {0, 0, 0, 0};
