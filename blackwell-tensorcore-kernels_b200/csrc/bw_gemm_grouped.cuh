@@ -99,31 +99,43 @@ __device__ __forceinline__ void mbar_drain(uint64_t* bar, uint32_t parity, uint6
 __device__ __forceinline__ void grouped_fetch(const int* offsets, int groups, int rows, int* bounds) {
   for (int g = threadIdx.x; g <= groups; g += kGroupedThreads) bounds[g] = min(max(__ldcg(offsets + g), 0), rows);
 }
+// Each lane takes a run of consecutive entries, so both scans cross the warp once whatever `groups` is
+// (32 groups at a time, 64 of them took about 1300 cycles).
 __device__ __forceinline__ void grouped_scan(int groups, int tm, int per_row, int* bounds, int* tiles) {
   const int lane = threadIdx.x & 31;
-  int high = 0, sum = 0;
-  for (int base = 0; base <= groups; base += 32) {
-    const int g = base + lane;
-    int v = g <= groups ? bounds[g] : 0;
+  const int run = groups / 32 + 1;  // of the groups + 1 bounds
+  const int first = min(lane * run, groups + 1), last = min(first + run, groups + 1);
+  int high = 0;  // largest bound of the run
+  for (int g = first; g < last; ++g) high = max(high, bounds[g]);
+  int before = high;
 #pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int u = __shfl_up_sync(0xffffffffu, v, o);
-      if (lane >= o) v = max(v, u);
-    }
-    v = max(v, high);
-    int before = __shfl_up_sync(0xffffffffu, v, 1);  // bounds[g - 1]
-    if (lane == 0) before = high;
-    high = __shfl_sync(0xffffffffu, v, 31);
-    if (g <= groups) bounds[g] = v;
-    if (tiles == nullptr) continue;
-    int n = g > 0 && g <= groups ? (v - before + tm - 1) / tm * per_row : 0;  // tiles of group g - 1
+  for (int o = 1; o < 32; o <<= 1) {
+    const int u = __shfl_up_sync(0xffffffffu, before, o);
+    if (lane >= o) before = max(before, u);
+  }
+  before = __shfl_up_sync(0xffffffffu, before, 1);  // largest bound in front of the run
+  if (lane == 0) before = 0;
+  int v = before, sum = 0;
+  for (int g = first; g < last; ++g) {
+    const int u = max(v, bounds[g]);
+    bounds[g] = u;
+    if (g > 0) sum += (u - v + tm - 1) / tm * per_row;  // tiles of group g - 1
+    v = u;
+  }
+  if (tiles == nullptr) return;
+  int at = sum;
 #pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int u = __shfl_up_sync(0xffffffffu, n, o);
-      if (lane >= o) n += u;
-    }
-    if (g <= groups) tiles[g] = sum + n;
-    sum += __shfl_sync(0xffffffffu, n, 31);
+  for (int o = 1; o < 32; o <<= 1) {
+    const int u = __shfl_up_sync(0xffffffffu, at, o);
+    if (lane >= o) at += u;
+  }
+  at -= sum;  // tiles in front of the run
+  v = before;
+  for (int g = first; g < last; ++g) {
+    const int u = bounds[g];
+    if (g > 0) at += (u - v + tm - 1) / tm * per_row;
+    tiles[g] = at;
+    v = u;
   }
 }
 
@@ -292,6 +304,11 @@ __device__ __forceinline__ int a_load_bytes(int valid) {
 // WGRAD: a slab with `left` rows of its group left ends inside a k-step of 16.
 __device__ __forceinline__ bool slab_is_cut(int left, int slab) { return left < slab && (left & 15) != 0; }
 
+// Groups of few rows: bound by HBM, which every weight leaves once (64 matrices of 4096 x 2048 E4M3, 16 rows each:
+// 85-90 us, 6.0-6.5 TB/s of the measured 6.5). Persistent, one CTA an SM: warp 0 streams k-slabs into
+// a ring of 3 to 10 stages, warp 1 multiplies, warps 2-5 store one tile while the next is summed in the
+// other half of Tensor Memory. A tile has 128 rows however few count: their products cost nothing while the weights
+// arrive, and narrower tiles would read them again.
 // One CTA a tile of 128 x W (W <= 256; a multiple of 16, for an N-contiguous B of 64).
 template <Kind KIND, GMode MODE, Out OUT>
 __global__ void __launch_bounds__(kGroupedThreads, 1)
@@ -530,7 +547,9 @@ __global__ void __launch_bounds__(kGroupedThreads, 1)
 }
 
 // ------------------------------------------------------------------------------------
-// CTA pairs: 256 x 256 tiles for groups with many rows. As in bw_gemm_pair.cuh, each CTA of a pair
+// CTA pairs: 256 x 256 tiles for groups with many rows, bound by the tensor cores (91-92% of the active cycles; 8 x
+// 4096 rows of 4096 x 2048 BF16 344 us = 1597 TFLOP/s at 1.48 GHz, E4M3 8 x 2048 of 8192 x 4096 360 us = 3057): a pair
+// moves a third less per product than two single CTAs, which L2 cannot feed at that rate. As in bw_gemm_pair.cuh, each CTA of a pair
 // loads its 128 rows of A and 128 columns of B, the leader's MMA thread multiplies both halves, and a
 // pipeline stage holds two swizzle atoms of K. Barriers: full[s], fixed[s] and accempty[b] count in
 // the leader; empty[s], accfull[b] and tailfull[s] exist in both CTAs.

@@ -146,6 +146,36 @@ def test_pitches_and_alignment(cuda_dev, cols, pad, shift, dtype):
         assert bool((whole == fill).all())
 
 
+@pytest.mark.parametrize("cols", [1, 5, 16, 300, 1500, 5000, 9000])
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+def test_tensors_of_different_alignment(cuda_dev, cols, dtype):
+    """Each tensor at a distance of its own from a vector's boundary: element by element."""
+    import torch
+
+    dt, rows = getattr(torch, dtype), 9
+
+    def place(src, shift, pad):
+        whole = torch.zeros(rows * (cols + pad) + 32, dtype=src.dtype, device=cuda_dev)
+        view = whole[shift:shift + rows * (cols + pad)].view(rows, cols + pad)[:, :cols]
+        view.copy_(src)
+        return view
+
+    x, r, w = _inputs(cuda_dev, dt, rows, cols, True)
+    wide = torch.zeros(cols + 3, dtype=dt, device=cuda_dev)
+    wide[3:] = w
+    xs, rs = place(x, 1, 3), place(r, 2, 1)
+    ys, hs, qs = place(x, 5, 0), place(x, 0, 8), place(x.to(torch.uint8), 3, 2)
+    y, h, rstd = bwgemm.rmsnorm(xs, wide[3:], residual=rs, eps=EPS, y=ys, h=hs)
+    _check_forward(x, r, w, y, h, rstd)
+    q, s, h, rstd = bwgemm.rmsnorm_fp8(xs, wide[3:], residual=rs, eps=EPS, q=qs, h=hs)
+    _check_fp8(x, r, w, q, s, h, rstd)
+    dx, dw = bwgemm.rmsnorm_backward(place(x, 7, 0), h, wide[3:], rstd, dresidual=rs, dx=place(x, 2, 5))
+    _check_backward(x, h, w, rstd, r, dx, dw)
+    # one alignment for all rows, the weights at another
+    y, h, rstd = bwgemm.rmsnorm(x, wide[3:], residual=r, eps=EPS)
+    _check_forward(x, r, w, y, h, rstd)
+
+
 def test_in_place(cuda_dev):
     """y over x, h over the residual, dx over dy: registers and long rows alike."""
     import torch
