@@ -23,7 +23,10 @@ namespace bw {
 enum class GMode : int { ROWS_NK = 0, ROWS_KN = 1, WGRAD = 2 };
 
 constexpr int kMaxGroups = 1024;
-constexpr int kGroupedThreads = 224;  // producer, MMA, 4 epilogue warps, tail warp
+constexpr int kGroupedEpiWarps = 8;   // two for each 32 lanes of Tensor Memory
+constexpr int kGroupedThreads = 32 * (2 + kGroupedEpiWarps + 1);  // producer, MMA, epilogue, tail warp
+constexpr int kGroupedChunkBytes = 64;                             // of a row, staged at a time
+constexpr int kGroupedStageBytes = 32 * kGroupedChunkBytes;        // staging of one epilogue warp
 constexpr int kGroupedMaxStages = 10;
 
 struct GroupedParams {
@@ -190,19 +193,31 @@ struct GWalk {
   }
 };
 
-// One warp's 32 rows x W columns of a finished accumulator (zeros where nothing was summed), 128
-// bytes of every row at a time: registers -> the warp's 4 KB of shared memory (16-byte pieces,
-// XOR-swizzled over the banks) -> 8 lanes a row, so that a store instruction covers whole 128-byte
-// lines. A lane storing its own row straight from registers touches 32 lines an instruction; tiles
-// that sum little (a gradient of few rows a group) are bound by that. `release` runs after the last
-// read of the accumulator.
+// TMEM -> registers: 32 lanes x 16 consecutive 32-bit columns.
+__device__ __forceinline__ void tmem_ld_32x32b_x16(uint32_t taddr, uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+      "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+        "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(taddr)
+      : "memory");
+}
+
+// One warp's share of 32 rows x W columns of a finished accumulator (zeros where nothing was summed): every other
+// chunk of 64 bytes of each row, from chunk `part`. A chunk goes registers -> the warp's 2 KB of shared memory
+// (16-byte pieces, XOR-swizzled over the banks) -> 4 lanes a row, so that a store instruction covers whole
+// sectors of 8 rows. A lane storing its own row straight from registers touches 32 lines an instruction; tiles that
+// sum little (a gradient of few rows a group, short K) are bound by that, and by the latency of one
+// warp's chain: hence two warps for the same rows. `release` runs after the last read of the accumulator.
 template <GMode MODE, Out OUT, typename Release>
 __device__ __forceinline__ void grouped_epilogue(const GroupedParams& p, const GTile& t, uint32_t tbase, int first,
-                                                 int lane, uint32_t stage, Release release) {
-  constexpr int kCols = OUT == Out::F32 ? 32 : 64;     // columns in 128 bytes
+                                                 int part, int lane, uint32_t stage, Release release) {
   constexpr int kElem = OUT == Out::F32 ? 4 : 2;
+  constexpr int kCols = kGroupedChunkBytes / kElem;    // columns of a chunk
   constexpr int kPiece = 16 / kElem;
-  if (first >= t.rows) {  // none of this warp's rows exists
+  const int width = min(p.W, p.n - t.col0);
+  if (first >= t.rows || part * kCols >= width) {  // none of this warp's rows or columns exists
     release();
     return;
   }
@@ -220,24 +235,24 @@ __device__ __forceinline__ void grouped_epilogue(const GroupedParams& p, const G
   }
   const long long pitch = p.ldc * kElem;
   char* out = static_cast<char*>(p.C) + row * pitch + static_cast<long long>(t.col0) * kElem;
-  const int width = min(p.W, p.n - t.col0);
   const bool summed = t.k > 0;
-  // the pieces that this lane stores: row rr + 4 i, piece jj (rows 4 apart alternate between two
-  // places of the swizzle)
-  const int rr = lane >> 3, jj = lane & 7;
-  const uint32_t from0 = stage + rr * 128 + ((jj ^ rr) << 4), from1 = stage + (rr + 4) * 128 + ((jj ^ (rr + 4)) << 4);
+  // the pieces that this lane stores: piece jj of rows rr + 8 i
+  const int rr = lane >> 2, jj = lane & 3;
+  const uint32_t from = stage + rr * kGroupedChunkBytes + ((jj ^ ((rr >> 1) & 3)) << 4);
+  const uint32_t to = stage + lane * kGroupedChunkBytes;
+  const int swz = (lane >> 1) & 3;
   uint32_t v[kCols];
   auto load = [&](int c) {
-    tmem_ld_32x32b_x32(tbase + c, *reinterpret_cast<uint32_t(*)[32]>(&v[0]));
-    if constexpr (kCols == 64) tmem_ld_32x32b_x32(tbase + c + 32, *reinterpret_cast<uint32_t(*)[32]>(&v[32]));
+    if constexpr (kCols == 32) tmem_ld_32x32b_x32(tbase + c, v);
+    else tmem_ld_32x32b_x16(tbase + c, v);
   };
-  if (summed) load(0);
+  if (summed) load(part * kCols);
 #pragma unroll 1
-  for (int c = 0; c < width; c += kCols) {
-    uint32_t w[32];
+  for (int c = part * kCols; c < width; c += 2 * kCols) {
+    uint32_t w[16];
     if (summed) tmem_ld_wait();
 #pragma unroll
-    for (int j = 0; j < 32; ++j) {
+    for (int j = 0; j < 16; ++j) {
       if constexpr (OUT == Out::F32) {
         w[j] = __float_as_uint(__uint_as_float(v[j]) * alpha);
       } else {
@@ -248,28 +263,27 @@ __device__ __forceinline__ void grouped_epilogue(const GroupedParams& p, const G
       if (!summed) w[j] = 0;
     }
     if (summed) {  // the next columns come while these are stored
-      if (c + kCols < width) load(c + kCols);
+      if (c + 2 * kCols < width) load(c + 2 * kCols);
       else release();
     }
 #pragma unroll
-    for (int j = 0; j < 8; ++j)
-      st_shared_v4(stage + lane * 128 + ((j ^ (lane & 7)) << 4), w[4 * j], w[4 * j + 1], w[4 * j + 2], w[4 * j + 3]);
+    for (int j = 0; j < 4; ++j) st_shared_v4(to + ((j ^ swz) << 4), w[4 * j], w[4 * j + 1], w[4 * j + 2], w[4 * j + 3]);
     __syncwarp();
     const int have = width - c - jj * kPiece;  // columns of this lane's pieces that exist
     char* dst = out + rr * pitch + (c + jj * kPiece) * kElem;
     if (p.vec == 16 && width - c >= kCols) {
-      uint4 x[8];
+      uint4 x[4];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) x[i] = ld_shared_v4((i & 1 ? from1 : from0) + (i >> 1) * 1024);
+      for (int i = 0; i < 4; ++i) x[i] = ld_shared_v4(from + i * 8 * kGroupedChunkBytes);
 #pragma unroll
-      for (int i = 0; i < 8; ++i)
-        if (rr + 4 * i < nrows) st_global_v4(dst + 4 * i * pitch, x[i]);
+      for (int i = 0; i < 4; ++i)
+        if (rr + 8 * i < nrows) st_global_v4(dst + 8 * i * pitch, x[i]);
     } else {
 #pragma unroll 1
-      for (int i = 0; i < 8; ++i) {
-        if (rr + 4 * i >= nrows || have <= 0) continue;
-        const uint4 x = ld_shared_v4((i & 1 ? from1 : from0) + (i >> 1) * 1024);
-        char* at = dst + 4 * i * pitch;
+      for (int i = 0; i < 4; ++i) {
+        if (rr + 8 * i >= nrows || have <= 0) continue;
+        const uint4 x = ld_shared_v4(from + i * 8 * kGroupedChunkBytes);
+        char* at = dst + 8 * i * pitch;
         if (p.vec == 16 && have >= kPiece) {
           st_global_v4(at, x);
         } else {
@@ -290,7 +304,7 @@ __device__ __forceinline__ void grouped_epilogue(const GroupedParams& p, const G
 __host__ __device__ constexpr int grouped_tail_bytes(int groups) {
   // barriers (full, empty, tailfull, fixed per stage; accfull, accempty x 2; teardown), TMEM slot and abort
   // flag, bounds and tiles, the epilogue's staging, alignment slack
-  return (4 * kGroupedMaxStages + 5) * 8 + 16 + 2 * (groups + 1) * 4 + kEpiWarps * kEpiBufBytes + 1024;
+  return (4 * kGroupedMaxStages + 5) * 8 + 16 + 2 * (groups + 1) * 4 + kGroupedEpiWarps * kGroupedStageBytes + 1024;
 }
 
 // A tile of few rows loads them in boxes of 16 (a box of 128 rows would fetch its neighbours' too, and
@@ -306,7 +320,7 @@ __device__ __forceinline__ bool slab_is_cut(int left, int slab) { return left < 
 
 // Groups of few rows: bound by HBM, which every weight leaves once (64 matrices of 4096 x 2048 E4M3, 16 rows each:
 // 85-90 us, 6.0-6.5 TB/s of the measured 6.5). Persistent, one CTA an SM: warp 0 streams k-slabs into
-// a ring of 3 to 10 stages, warp 1 multiplies, warps 2-5 store one tile while the next is summed in the
+// a ring of 3 to 10 stages, warp 1 multiplies, warps 2-9 store one tile while the next is summed in the
 // other half of Tensor Memory. A tile has 128 rows however few count: their products cost nothing while the weights
 // arrive, and narrower tiles would read them again.
 // One CTA a tile of 128 x W (W <= 256; a multiple of 16, for an N-contiguous B of 64).
@@ -325,7 +339,7 @@ __global__ void __launch_bounds__(kGroupedThreads, 1)
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   const int S = p.stages;
   uint8_t* staging = smem + static_cast<size_t>(S) * p.stage_bytes;
-  uint64_t* full = reinterpret_cast<uint64_t*>(staging + kEpiWarps * kEpiBufBytes);
+  uint64_t* full = reinterpret_cast<uint64_t*>(staging + kGroupedEpiWarps * kGroupedStageBytes);
   uint64_t* empty = full + kGroupedMaxStages;
   uint64_t* tailfull = empty + kGroupedMaxStages;  // WGRAD: a cut slab has landed, its rows behind the end still to clear
   uint64_t* fixed = tailfull + kGroupedMaxStages;  // ... and are cleared
@@ -347,7 +361,7 @@ __global__ void __launch_bounds__(kGroupedThreads, 1)
       mbar_init(&tailfull[s], 1);
       mbar_init(&fixed[s], 1);
     }
-    for (int b = 0; b < 2; ++b) { mbar_init(&accfull[b], 1); mbar_init(&accempty[b], kEpiWarps * 32); }
+    for (int b = 0; b < 2; ++b) { mbar_init(&accfull[b], 1); mbar_init(&accempty[b], kGroupedEpiWarps * 32); }
     mbar_init(teardown, 1);
     *abort_flag = 0;
     fence_mbar_init();
@@ -487,15 +501,15 @@ __global__ void __launch_bounds__(kGroupedThreads, 1)
       umma_commit(teardown);
       mbar_drain(teardown, 0, p.budget_ns);
     }
-  } else if (warp < 6) {
+  } else if (warp < 2 + kGroupedEpiWarps) {
     // ---------------- epilogue ----------------
-    const int q = warp & 3;
-    const uint32_t stage = smem_u32(staging) + q * kEpiBufBytes;
+    const int q = warp & 3, part = (warp - 2) >> 2;  // lanes of Tensor Memory, every other chunk of columns
+    const uint32_t stage = smem_u32(staging) + (warp - 2) * kGroupedStageBytes;
     int local = 0;
     for (int t = blockIdx.x; t < num_tiles; t += gridDim.x) {
       const GTile o = walk.at(t);
       if (o.k == 0) {
-        grouped_epilogue<MODE, OUT>(p, o, 0, q * 32, lane, stage, [] {});
+        grouped_epilogue<MODE, OUT>(p, o, 0, q * 32, part, lane, stage, [] {});
         continue;
       }
       const int b = local & 1;
@@ -503,7 +517,7 @@ __global__ void __launch_bounds__(kGroupedThreads, 1)
       ++local;
       if (!mbar_wait_warp(&accfull[b], aph, wc, 25)) break;
       tc_fence_after();
-      grouped_epilogue<MODE, OUT>(p, o, tmem_base + (static_cast<uint32_t>(q * 32) << 16) + b * 256, q * 32, lane, stage,
+      grouped_epilogue<MODE, OUT>(p, o, tmem_base + (static_cast<uint32_t>(q * 32) << 16) + b * 256, q * 32, part, lane, stage,
                                   [&] {
                                     tc_fence_before();
                                     mbar_arrive(&accempty[b]);
@@ -602,7 +616,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGroupedThreads, 1)
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* staging = smem + S * kPairStageBytes;
-  uint64_t* full = reinterpret_cast<uint64_t*>(staging + kEpiWarps * kEpiBufBytes);
+  uint64_t* full = reinterpret_cast<uint64_t*>(staging + kGroupedEpiWarps * kGroupedStageBytes);
   uint64_t* empty = full + kGroupedMaxStages;
   uint64_t* tailfull = empty + kGroupedMaxStages;
   uint64_t* fixed = tailfull + kGroupedMaxStages;
@@ -628,7 +642,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGroupedThreads, 1)
       mbar_init(&tailfull[s], 1);
       mbar_init(&fixed[s], 2);
     }
-    for (int b = 0; b < 2; ++b) { mbar_init(&accfull[b], 1); mbar_init(&accempty[b], 2 * kEpiWarps); }
+    for (int b = 0; b < 2; ++b) { mbar_init(&accfull[b], 1); mbar_init(&accempty[b], 2 * kGroupedEpiWarps); }
     mbar_init(teardown, 1);
     *abort_flag = 0;
     fence_mbar_init();
@@ -781,16 +795,16 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGroupedThreads, 1)
       umma_commit_pair(smem_u32(teardown));
       mbar_drain(teardown, 0, p.budget_ns);
     }
-  } else if (warp < 6) {
+  } else if (warp < 2 + kGroupedEpiWarps) {
     // ---------------- epilogue (both CTAs) ----------------
-    const int q = warp & 3;
+    const int q = warp & 3, part = (warp - 2) >> 2;  // lanes of Tensor Memory, every other chunk of columns
     const uint32_t accempty_leader = mapa_shared(smem_u32(accempty), 0);
-    const uint32_t stage = smem_u32(staging) + q * kEpiBufBytes;
+    const uint32_t stage = smem_u32(staging) + (warp - 2) * kGroupedStageBytes;
     int local = 0;
     for (int t = cluster; t < num_tiles; t += nclusters) {
       const GTile o = walk.at(t);
       if (o.k == 0) {
-        grouped_epilogue<MODE, OUT>(p, o, 0, half + q * 32, lane, stage, [] {});
+        grouped_epilogue<MODE, OUT>(p, o, 0, half + q * 32, part, lane, stage, [] {});
         continue;
       }
       const int b = local & 1;
@@ -798,8 +812,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGroupedThreads, 1)
       ++local;
       if (!mbar_wait_warp(&accfull[b], aph, wc, 65)) break;
       tc_fence_after();
-      grouped_epilogue<MODE, OUT>(p, o, tmem_base + (static_cast<uint32_t>(q * 32) << 16) + b * 256, half + q * 32, lane,
-                                  stage, [&] {
+      grouped_epilogue<MODE, OUT>(p, o, tmem_base + (static_cast<uint32_t>(q * 32) << 16) + b * 256, half + q * 32, part,
+                                  lane, stage, [&] {
                                     tc_fence_before();
                                     __syncwarp();
                                     if (lane == 0) mbar_arrive_remote_cta(accempty_leader + b * 8);

@@ -821,8 +821,8 @@ int norm_impl(const void* x, long long ldx, const void* residual, long long ldr,
 
 // Slabs of the weight gradient, one a block: a function of the sizes alone, so that the sums (and the
 // workspace) are the same on every device. 512 threads are resident on an SM (of 148) with this
-// kernel's registers, and a block has one for 16 columns, or 256 for short rows; more slabs wait for a
-// second round and write more partial sums (16384 x 8192 BF16: 180 us with 148, 185 with 296, 199 with 592).
+// kernel's registers, and a block has one for 16 columns, or 256 for short rows; more slabs wait for
+// those to end and write more partial sums (16384 x 8192 BF16: 180 us with 148, 185 with 296, 199 with 592).
 int grad_slabs(long long rows, long long cols) {
   long long most = 296;
   if (cols > 512 && cols <= 16384) most = 148LL * 512 / (cols > 8192 ? 512 : (cols + 511) / 512 * 32);
