@@ -315,6 +315,14 @@ __device__ __forceinline__ int a_load_bytes(int valid) {
   return valid > kFewRows ? kBM * kSlabBytes : (valid + 15) / 16 * 16 * kSlabBytes;
 }
 
+// Clears n (1..15) rows of 128 bytes: a warp, 4 rows at a time.
+__device__ __forceinline__ void clear_rows(uint32_t at, int n, int lane) {
+  const uint32_t mine = at + (lane >> 3) * kSlabBytes + (lane & 7) * 16;
+#pragma unroll
+  for (int r = 0; r < 16; r += 4)
+    if ((lane >> 3) + r < n) st_shared_v4(mine + r * kSlabBytes, 0, 0, 0, 0);
+}
+
 // WGRAD: a slab with `left` rows of its group left ends inside a k-step of 16.
 __device__ __forceinline__ bool slab_is_cut(int left, int slab) { return left < slab && (left & 15) != 0; }
 
@@ -539,12 +547,9 @@ __global__ void __launch_bounds__(kGroupedThreads, 1)
       const uint32_t base = smem_u32(smem + static_cast<size_t>(s) * p.stage_bytes);
       const int j = left / KA, at = left - j * KA;  // atom and row of the first row behind the end
       const uint32_t a0 = base + j * kABytes, b0 = base + p.sub * kABytes + j * b_bytes;
-      const int nz = ((left + 15) & ~15) - left;    // 1..15 rows of 128 bytes in each box
-      for (int i = lane; i < (2 + p.W / 64) * nz * 8; i += 32) {
-        const int box = i / (nz * 8), rest = i - box * nz * 8;
-        st_shared_v4((box < 2 ? a0 + box * kBoxBytes : b0 + (box - 2) * kBoxBytes) + (at + rest / 8) * kSlabBytes +
-                         (rest & 7) * 16, 0, 0, 0, 0);
-      }
+      const int nz = ((left + 15) & ~15) - left;    // 1..15 rows in each box
+      for (int box = 0; box < 2; ++box) clear_rows(a0 + box * kBoxBytes + at * kSlabBytes, nz, lane);
+      for (int box = 0; box < p.W / 64; ++box) clear_rows(b0 + box * kBoxBytes + at * kSlabBytes, nz, lane);
       fence_proxy_async_smem();
       __syncwarp();
       if (lane == 0) mbar_arrive(&fixed[s]);
@@ -834,12 +839,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGroupedThreads, 1)
       if (!mbar_wait_warp(&tailfull[s], (cut_ph >> s) & 1u, wc, 66)) break;
       cut_ph ^= 1u << s;
       const int j = left / KA, at = left - j * KA;  // atom and row of the first row behind the end
-      const uint32_t base = smem_u32(smem + s * kPairStageBytes) + j * kPairAtom;
+      const uint32_t base = smem_u32(smem + s * kPairStageBytes) + j * kPairAtom + at * kSlabBytes;
       const int nz = ((left + 15) & ~15) - left;
-      for (int i = lane; i < 4 * nz * 8; i += 32) {  // boxes: A, A + 64 columns, B, B + 64 columns
-        const int box = i / (nz * 8), rest = i - box * nz * 8;
-        st_shared_v4(base + (box >> 1) * kPairSub * kPairAtom + (box & 1) * kBoxBytes + (at + rest / 8) * kSlabBytes +
-                         (rest & 7) * 16, 0, 0, 0, 0);
+#pragma unroll
+      for (int box = 0; box < 2; ++box) {
+        clear_rows(base + box * kBoxBytes, nz, lane);                          // A
+        clear_rows(base + kPairSub * kPairAtom + box * kBoxBytes, nz, lane);  // B
       }
       fence_proxy_async_smem();
       __syncwarp();
