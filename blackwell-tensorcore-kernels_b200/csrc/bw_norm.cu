@@ -13,8 +13,8 @@
 // reduction and its output. max |y| needs no second reduction: y_j = (h_j w_j) rstd and rounding is
 // monotonic, so max |y| = max |h w| * rstd exactly, and both sums travel through one reduction.
 // Statistics and sums are FP32. Measured, 16384 x 8192 BF16 with residual: to E4M3 140 us (6.7 TB/s of
-// the 7 bytes an element), gradient 175 us (6.1 TB/s of 8 bytes); 131072 x 128 BF16 to BF16 10.5 us
-// (6.4 TB/s); 8192 x 4095 to E4M3, rows at every alignment, 50 us; one row of 8192 2.8 us.
+// the 7 bytes an element), gradient 155 us (6.9 TB/s of 8 bytes); 131072 x 128 BF16 to BF16 10.5 us
+// (6.4 TB/s); 16384 x 8191 to E4M3, rows at every alignment, 144 us; one row of 8192 2.8 us.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_fp8.h>
@@ -111,6 +111,34 @@ __device__ __forceinline__ float elem(const Words<BYTES>& v, int j) {
     return __uint_as_float(j & 1 ? v.u[j / 2] & 0xffff0000u : v.u[j / 2] << 16);
   }
 }
+// Two FP32 operations an instruction (these kernels issue 5 to 10 instructions an element, enough to
+// show beside the memory's time).
+__device__ __forceinline__ uint64_t pack2(float2 a) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a.x), "f"(a.y));
+  return r;
+}
+__device__ __forceinline__ float2 unpack2(uint64_t r) {
+  float2 a;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(a.x), "=f"(a.y) : "l"(r));
+  return a;
+}
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(pack2(a)), "l"(pack2(b)));
+  return unpack2(r);
+}
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(pack2(a)), "l"(pack2(b)), "l"(pack2(c)));
+  return unpack2(r);
+}
+// Elements 2 i and 2 i + 1.
+template <typename T, int BYTES>
+__device__ __forceinline__ float2 elems2(const Words<BYTES>& v, int i) {
+  if constexpr (std::is_same_v<T, __half>) return __half22float2(*reinterpret_cast<const __half2*>(&v.u[i]));
+  else return make_float2(elem<T>(v, 2 * i), elem<T>(v, 2 * i + 1));
+}
 template <typename T>
 __device__ __forceinline__ uint32_t two_elems(float a, float b) {
   if constexpr (std::is_same_v<T, __half>) {
@@ -200,21 +228,32 @@ __device__ __forceinline__ Vec<WT, VE> load_weight(const void* w, const Columns<
 struct SumMax {
   float sum, max;
 };
+template <bool MAX>
 __device__ __forceinline__ SumMax reduce_lanes(SumMax v, int width) {
   for (int o = width / 2; o > 0; o >>= 1) {
     v.sum += __shfl_xor_sync(0xffffffffu, v.sum, o);
-    v.max = fmaxf(v.max, __shfl_xor_sync(0xffffffffu, v.max, o));
+    if constexpr (MAX) v.max = fmaxf(v.max, __shfl_xor_sync(0xffffffffu, v.max, o));
   }
   return v;
 }
+// The whole warp: maxima of magnitudes order as integers.
+template <bool MAX>
+__device__ __forceinline__ SumMax reduce_warp(SumMax v) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v.sum += __shfl_xor_sync(0xffffffffu, v.sum, o);
+  if constexpr (MAX) v.max = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(v.max)));
+  return v;
+}
+template <bool MAX>
 __device__ __forceinline__ SumMax reduce_row(SumMax v, int tpr, SumMax* sm) {
-  v = reduce_lanes(v, tpr < 32 ? tpr : 32);
+  if (tpr < 32) return reduce_lanes<MAX>(v, tpr);
+  v = reduce_warp<MAX>(v);
   if (tpr > 32) {
     const int warps = tpr >> 5, lane = threadIdx.x & 31;
     if (lane == 0) sm[threadIdx.x >> 5] = v;
     __syncthreads();
     v = lane < warps ? sm[lane] : SumMax{0.f, 0.f};  // maxima are of magnitudes
-    v = reduce_lanes(v, 32);
+    v = reduce_warp<MAX>(v);
   }
   return v;
 }
@@ -231,8 +270,11 @@ struct NormParams {
   long long ldx, ldr, ldh, ldy;  // row pitches in elements
   long long rows;
   int cols;
-  float eps;
+  float eps, inv_cols;
   int phase;           // elements between a vector's boundary and the first row (SHIFT)
+  int depth;           // rows in flight (staged kernels)
+  int* status;
+  unsigned long long budget_ns;
 };
 
 // Scale of an E4M3 row by its maximum, and the factor that quantises it. A maximum so small that
@@ -241,10 +283,24 @@ __device__ __forceinline__ void e4m3_row_scale(float amax, float& mul, float& s)
   mul = 1.f;
   s = 1.f;
   if (amax > 0.f && amax < INFINITY) {
-    const float m = kE4m3Max / amax;
+    const float m = amax < 0x1p125f ? __fdividef(kE4m3Max, amax) : kE4m3Max / amax;  // the former gives 0 from 2^126 on
     if (m < INFINITY) {
       mul = m;
       s = amax / kE4m3Max;
+    }
+  }
+}
+
+template <int VE>
+__device__ __forceinline__ void scale(const float (&a)[VE], float f, float (&o)[VE]) {
+  if constexpr (VE == 1) {
+    o[0] = a[0] * f;
+  } else {
+#pragma unroll
+    for (int j = 0; j < VE; j += 2) {
+      const float2 q = mul2(make_float2(a[j], a[j + 1]), make_float2(f, f));
+      o[j] = q.x;
+      o[j + 1] = q.y;
     }
   }
 }
@@ -256,7 +312,7 @@ __device__ __forceinline__ Words<VE> encode_e4m3(const float (&y)[VE], float mul
 #pragma unroll
     for (int j = 0; j < VE; j += 2) {
       const __nv_fp8x2_storage_t two =
-          __nv_cvt_float2_to_fp8x2(make_float2(y[j] * mul, y[j + 1] * mul), __NV_SATFINITE, __NV_E4M3);
+          __nv_cvt_float2_to_fp8x2(mul2(make_float2(y[j], y[j + 1]), make_float2(mul, mul)), __NV_SATFINITE, __NV_E4M3);
       q.u[j / 4] |= static_cast<uint32_t>(two) << (8 * (j % 4));
     }
   } else {
@@ -265,31 +321,67 @@ __device__ __forceinline__ Words<VE> encode_e4m3(const float (&y)[VE], float mul
   return q;
 }
 
-template <typename T, int VE>
+// h + r, rounded once. Through FP32 the 16-bit result is the same (where the FP32 sum rounds, the smaller
+// term is too small to matter to the 16-bit one either), takes 7 instructions for 2 elements instead of 1, and is
+// what PACKED = false asks for.
+template <typename T, int VE, bool PACKED = true>
 __device__ __forceinline__ void add_residual(Vec<T, VE>& h, const Vec<T, VE>& r) {
-  float f[VE];
+  if constexpr (!PACKED || std::is_same_v<T, float>) {
+    float f[VE];
 #pragma unroll
-  for (int j = 0; j < VE; ++j) f[j] = elem<T>(h, j) + elem<T>(r, j);
-  h = from_floats<T, VE>(f);
+    for (int j = 0; j < VE; ++j) f[j] = elem<T>(h, j) + elem<T>(r, j);
+    h = from_floats<T, VE>(f);
+  } else {
+    using T2 = std::conditional_t<std::is_same_v<T, __half>, __half2, __nv_bfloat162>;
+#pragma unroll
+    for (int i = 0; i < static_cast<int>(sizeof(h.u) / 4); ++i) {
+      const T2 sum = __hadd2(*reinterpret_cast<const T2*>(&h.u[i]), *reinterpret_cast<const T2*>(&r.u[i]));
+      h.u[i] = *reinterpret_cast<const uint32_t*>(&sum);
+    }
+  }
+}
+__device__ __forceinline__ float add_as(float, float a, float b) { return a + b; }
+template <typename T>
+__device__ __forceinline__ float add_as(T, float a, float b) {
+  return to_f32(__hadd(from_f32<T>(a), from_f32<T>(b)));
 }
 
 // p = h w, and its share of the row's sums.
 template <bool Q8, typename T, typename WT, int VE>
 __device__ __forceinline__ void accumulate(const Vec<T, VE>& h, const Vec<WT, VE>& w, float (&p)[VE], SumMax& a) {
-#pragma unroll
-  for (int j = 0; j < VE; ++j) {
-    const float v = elem<T>(h, j);
-    p[j] = v * elem<WT>(w, j);
+  if constexpr (VE == 1) {
+    const float v = elem<T>(h, 0);
+    p[0] = v * elem<WT>(w, 0);
     a.sum = fmaf(v, v, a.sum);
-    if constexpr (Q8) a.max = fmaxf(a.max, fabsf(p[j]));
+    if constexpr (Q8) a.max = fmaxf(a.max, fabsf(p[0]));
+  } else {
+    float2 s = make_float2(0.f, 0.f);
+#pragma unroll
+    for (int i = 0; i < VE / 2; ++i) {
+      const float2 v = elems2<T>(h, i);
+      const float2 q = mul2(v, elems2<WT>(w, i));
+      s = fma2(v, v, s);
+      if constexpr (Q8) a.max = fmaxf(fmaxf(a.max, fabsf(q.x)), fabsf(q.y));
+      p[2 * i] = q.x;
+      p[2 * i + 1] = q.y;
+    }
+    a.sum += s.x + s.y;
   }
+}
+
+// v^(-1/2): CUDA's rsqrtf (2 steps off at most) and a Newton step. All threads of a row take it, in front of
+// their output: a square root and a division are 40 instructions more.
+__device__ __forceinline__ float inv_sqrt(float v) {
+  const float y = rsqrtf(v);
+  const float better = fmaf(0.5f * y, fmaf(-v * y, y, 1.f), y);
+  return better < INFINITY && better > 0.f ? better : y;  // v = 0, infinite, NaN or so small that a product overflows
 }
 
 // Writes a row's rstd (and scale). Returns the factor from h w to y, or to the code's value; where that
 // overflows (a row of tiny values), `pre` is a first factor of its own, else 1.
 template <bool Q8>
 __device__ __forceinline__ float finish_row(const NormParams& p, long long row, const SumMax& a, bool first, float& pre) {
-  const float rstd = 1.f / sqrtf(a.sum / static_cast<float>(p.cols) + p.eps);
+  const float rstd = inv_sqrt(fmaf(a.sum, p.inv_cols, p.eps));
   float mul = 1.f, s = 1.f;
   if constexpr (Q8) e4m3_row_scale(a.max * rstd, mul, s);
   if (first) {
@@ -313,8 +405,7 @@ __device__ __forceinline__ auto output(const float (&hw)[VE], float f, float pre
     return encode_e4m3<VE>(y, f);
   } else {
     float y[VE];
-#pragma unroll
-    for (int j = 0; j < VE; ++j) y[j] = hw[j] * f;
+    scale<VE>(hw, f, y);
     return from_floats<T, VE>(y);
   }
 }
@@ -332,6 +423,9 @@ constexpr int kThreadBytes = NV * (sizeof(T) * VE < 4 ? 4 : sizeof(T) * VE);
 template <typename T, typename WT, bool Q8, int VE, int NV, bool SHIFT>
 __global__ void __launch_bounds__(512) k_rmsnorm(const NormParams p, int tpr) {
   constexpr bool kKeep = kThreadBytes<T, VE, NV> <= 64;
+  // 16384 x 8192 BF16 140 us unpacked and 149 packed (the memory serves slower readers better), 4096 x 4096 20.3 / 19.5;
+  // in every other case packed is 2-12% faster
+  constexpr bool kPacked = SHIFT || NV != 4;
   grid_dependency_wait();
   __shared__ SumMax sm[2][32];
   const int per_block = blockDim.x / tpr;
@@ -366,8 +460,8 @@ __global__ void __launch_bounds__(512) k_rmsnorm(const NormParams p, int tpr) {
       if constexpr (!kKeep) fetch(row);
       if (r) {
 #pragma unroll
-        for (int i = 0; i < NV; ++i) add_residual<T, VE>(h.v[i], res.v[i]);
-        if constexpr (SHIFT) h.one = to_f32(from_f32<T>(h.one + res.one));
+        for (int i = 0; i < NV; ++i) add_residual<T, VE, kPacked>(h.v[i], res.v[i]);
+        if constexpr (SHIFT) h.one = add_as(T{}, h.one, res.one);
       }
       if (p.h) store_row(static_cast<T*>(p.h) + row * p.ldh, c, h);
 #pragma unroll
@@ -382,7 +476,7 @@ __global__ void __launch_bounds__(512) k_rmsnorm(const NormParams p, int tpr) {
       }
       if constexpr (kKeep) fetch(row + stride);
     }
-    a = reduce_row(a, tpr, sm[half]);
+    a = reduce_row<Q8>(a, tpr, sm[half]);
     half ^= 1;
     if (live) {
       float pre;
@@ -395,6 +489,138 @@ __global__ void __launch_bounds__(512) k_rmsnorm(const NormParams p, int tpr) {
         const float one[1] = {hw1};
         if (c.single >= 0) store_words<sizeof(O)>(y + c.single, output<T, Q8, 1>(one, f, pre));
       }
+    }
+  }
+}
+
+// Rows on their way to a block: the whole vectors of TENSORS rows a slot, `depth` slots, copied by the TMA unit while
+// the block is at earlier rows. So the bytes in flight depend neither on registers nor on idle lanes. One
+// thread of the row's own issues the copies (a warp for that alone takes the place of one that
+// computes: 37476 x 3519 gradient 208 us, 241 with such a warp).
+constexpr int kMaxDepth = 4;
+template <int TENSORS>  // of which the last may be absent
+struct RowRing {
+  uint64_t* full;   // [depth], shared
+  uint8_t* data;
+  int depth, pitch;  // bytes between the rows of a slot
+  int slot = 0;
+  uint32_t parity = 0;
+  const char* src[TENSORS];        // null: absent
+  long long step[TENSORS];         // bytes between a block's rows
+  uint32_t bytes;
+
+  __device__ __forceinline__ int tensors() const { return src[TENSORS - 1] ? TENSORS : TENSORS - 1; }
+  __device__ __forceinline__ uint8_t* at(int s, int tensor) const { return data + (s * tensors() + tensor) * pitch; }
+  __device__ __forceinline__ void issue(int s, long long n) const {  // the block's n-th row
+    mbar_arrive_expect_tx(&full[s], tensors() * bytes);
+#pragma unroll
+    for (int i = 0; i < TENSORS; ++i)
+      if (src[i] && bytes) bulk_load(at(s, i), src[i] + n * step[i], bytes, &full[s]);
+  }
+  __device__ __forceinline__ void advance() {
+    if (++slot == depth) { slot = 0; parity ^= 1; }
+  }
+};
+template <typename T, int VE, int NV, bool SHIFT>
+__device__ __forceinline__ void load_staged(const uint8_t* row, const Columns<VE, SHIFT>& c, Part<T, VE, NV, SHIFT>& o) {
+#pragma unroll
+  for (int i = 0; i < NV; ++i)
+    o.v[i] = c.has(i) ? load_words<sizeof(T) * VE>(row + (i * c.tpr + c.t) * (sizeof(T) * VE)) : zero_words<sizeof(T) * VE>();
+}
+
+// k_rmsnorm for rows over 128 vectors which leave lanes idle there, which start behind a boundary, or which are
+// too long for its registers: a block takes one row at a time out of its ring. Both measured, us, in registers / staged
+// (BF16 to E4M3 with residual): 23763 x 1088 39 / 36, 19407 x 2498 75 / 59, 10000 x 5000 67 / 56, 3564 x 9553 78 / 40; rows that
+// fill the lanes: 16384 x 8192 140 / 163, 32768 x 4000 140 / 160.
+template <typename T, typename WT, bool Q8, int VE, int NV, bool SHIFT>
+__global__ void __launch_bounds__(512) k_rmsnorm_staged(const NormParams p) {
+  constexpr bool kKeep = kThreadBytes<T, VE, NV> <= 64;
+  extern __shared__ __align__(128) uint8_t ring_data[];
+  __shared__ uint64_t full[kMaxDepth];
+  __shared__ int abort_flag;
+  __shared__ SumMax sm[2][32];
+  const int tpr = blockDim.x, t = threadIdx.x;
+  const long long stride = gridDim.x;
+  long long row = blockIdx.x;
+  const Columns<VE, SHIFT> c(tpr, t, static_cast<int>((p.phase + row * p.ldx) & (VE - 1)), p.cols);
+  const T* x = static_cast<const T*>(p.x);
+  const T* r = static_cast<const T*>(p.res);
+  RowRing<2> ring;
+  ring.full = full;
+  ring.data = ring_data;
+  ring.depth = p.depth;
+  ring.pitch = p.cols / VE * 16;
+  ring.src[0] = reinterpret_cast<const char*>(x + row * p.ldx + c.front);
+  ring.src[1] = r ? reinterpret_cast<const char*>(r + row * p.ldr + c.front) : nullptr;
+  ring.step[0] = stride * p.ldx * sizeof(T);
+  ring.step[1] = stride * p.ldr * sizeof(T);
+  ring.bytes = c.vecs * 16;
+  const WaitCtl wc{&abort_flag, p.status, p.budget_ns};
+  if (t == 0) {
+    for (int d = 0; d < p.depth; ++d) mbar_init(&full[d], 1);
+    abort_flag = 0;
+    fence_mbar_init();
+  }
+  grid_dependency_wait();
+  if (t == 0)
+    for (int d = 0; d < p.depth && row + d * stride < p.rows; ++d) ring.issue(d, d);
+  using O = std::conditional_t<Q8, uint8_t, T>;
+  Part<T, VE, NV, SHIFT> h, res;
+  Vec<WT, VE> w[kKeep ? NV : 1];
+  float w1 = 0.f, one = 0.f, one_res = 0.f;
+  auto fetch_single = [&](long long rw) {
+    if (!SHIFT || c.single < 0 || rw >= p.rows) return;
+    one = to_f32(x[rw * p.ldx + c.single]);
+    if (r) one_res = to_f32(r[rw * p.ldr + c.single]);
+  };
+  fetch_single(row);
+  if constexpr (kKeep) {
+#pragma unroll
+    for (int i = 0; i < NV; ++i) w[i] = load_weight<WT, VE, SHIFT>(p.w, c, i);
+  }
+  if (SHIFT && c.single >= 0) w1 = to_f32(static_cast<const WT*>(p.w)[c.single]);
+  __syncthreads();  // the barriers are set up
+  int half = 0;
+  for (long long n = 0; row < p.rows; ++n, row += stride) {
+    float hw[NV][VE], hw1 = 0.f;
+    SumMax a{0.f, 0.f};
+    mbar_wait(&full[ring.slot], ring.parity, wc, 71);  // after a timeout the block goes on, with wrong values and the status set
+    load_staged(ring.at(ring.slot, 0), c, h);
+    if (r) {
+      load_staged(ring.at(ring.slot, 1), c, res);
+#pragma unroll
+      for (int i = 0; i < NV; ++i) add_residual<T, VE>(h.v[i], res.v[i]);
+    }
+    if constexpr (SHIFT) {
+      h.one = r ? add_as(T{}, one, one_res) : one;
+      fetch_single(row + stride);
+    }
+    if (p.h) store_row(static_cast<T*>(p.h) + row * p.ldh, c, h);
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      if constexpr (!kKeep) w[0] = load_weight<WT, VE, SHIFT>(p.w, c, i);
+      accumulate<Q8, T, WT, VE>(h.v[i], w[kKeep ? i : 0], hw[i], a);
+    }
+    if constexpr (SHIFT) {
+      hw1 = h.one * w1;
+      a.sum = fmaf(h.one, h.one, a.sum);
+      if constexpr (Q8) a.max = fmaxf(a.max, fabsf(hw1));
+    }
+    __syncwarp();
+    a = reduce_row<Q8>(a, tpr, sm[half]);
+    half ^= 1;
+    // every thread has read its part of the slot
+    if (t == 0 && row + p.depth * stride < p.rows) ring.issue(ring.slot, n + p.depth);
+    ring.advance();
+    float pre;
+    const float f = finish_row<Q8>(p, row, a, t == 0, pre);
+    O* y = static_cast<O*>(p.y) + row * p.ldy;
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+      if (c.has(i)) store_words<sizeof(O) * VE>(y + c.col(i), output<T, Q8, VE>(hw[i], f, pre));
+    if constexpr (SHIFT) {
+      const float last[1] = {hw1};
+      if (c.single >= 0) store_words<sizeof(O)>(y + c.single, output<T, Q8, 1>(last, f, pre));
     }
   }
 }
@@ -418,7 +644,7 @@ __global__ void __launch_bounds__(1024) k_rmsnorm_wide(const NormParams p) {
     if (hr) store_words<sizeof(T) * VE>(hr + c, h);
     accumulate<Q8, T, WT, VE>(h, load_words<sizeof(WT) * VE>(w + c), hw, a);
   }
-  a = reduce_row(a, 1024, sm);
+  a = reduce_row<Q8>(a, 1024, sm);
   float pre;
   const float f = finish_row<Q8>(p, row, a, threadIdx.x == 0, pre);
   for (long long c = static_cast<long long>(threadIdx.x) * VE; c < p.cols; c += 1024LL * VE) {
@@ -454,7 +680,61 @@ struct NormGradParams {
   int cols;
   int slabs;           // blocks (each adds up the rows it takes)
   int phase;           // elements between a vector's boundary and the first row (SHIFT)
+  int depth;           // rows in flight (staged kernels)
+  int* status;
+  unsigned long long budget_ns;
 };
+
+// A vector's share of sum(g h) and of the weight gradient.
+template <typename T, typename WT, int VE>
+__device__ __forceinline__ void grad_sums(const Vec<T, VE>& dy, const Vec<T, VE>& h, const Vec<WT, VE>& w, float rstd,
+                                          float& sum, float (&dw)[VE]) {
+  if constexpr (VE == 1) {
+    const float d = elem<T>(dy, 0), v = elem<T>(h, 0);
+    sum = fmaf(d * elem<WT>(w, 0), v, sum);
+    dw[0] = fmaf(d * rstd, v, dw[0]);
+  } else {
+    float2 s = make_float2(0.f, 0.f);
+#pragma unroll
+    for (int i = 0; i < VE / 2; ++i) {
+      const float2 d = elems2<T>(dy, i), v = elems2<T>(h, i);
+      s = fma2(mul2(d, elems2<WT>(w, i)), v, s);
+      const float2 t = fma2(mul2(d, make_float2(rstd, rstd)), v, make_float2(dw[2 * i], dw[2 * i + 1]));
+      dw[2 * i] = t.x;
+      dw[2 * i + 1] = t.y;
+    }
+    sum += s.x + s.y;
+  }
+}
+template <typename T, typename WT, int VE>
+__device__ __forceinline__ Vec<T, VE> grad_output(const Vec<T, VE>& dy, const Vec<T, VE>& h, const Vec<WT, VE>& w,
+                                                  const Vec<T, VE>& dres, float rstd, float m) {
+  float o[VE];
+  if constexpr (VE == 1) {
+    o[0] = fmaf(rstd, fmaf(-m, elem<T>(h, 0) * rstd, elem<T>(dy, 0) * elem<WT>(w, 0)), elem<T>(dres, 0));
+  } else {
+    const float2 r2 = make_float2(rstd, rstd), m2 = make_float2(-m, -m);
+#pragma unroll
+    for (int i = 0; i < VE / 2; ++i) {
+      const float2 g = mul2(elems2<T>(dy, i), elems2<WT>(w, i)), n = mul2(elems2<T>(h, i), r2);
+      const float2 t = fma2(r2, fma2(m2, n, g), elems2<T>(dres, i));
+      o[2 * i] = t.x;
+      o[2 * i + 1] = t.y;
+    }
+  }
+  return from_floats<T, VE>(o);
+}
+
+template <int VE>
+__device__ __forceinline__ void store_sums(float* at, const float (&dw)[VE]) {
+  if (VE % 4 == 0 && (reinterpret_cast<uintptr_t>(at) & 15) == 0) {
+#pragma unroll
+    for (int j = 0; j + 3 < VE; j += 4) *reinterpret_cast<float4*>(at + j) = make_float4(dw[j], dw[j + 1], dw[j + 2], dw[j + 3]);
+  } else {
+#pragma unroll
+    for (int j = 0; j < VE; ++j) at[j] = dw[j];
+  }
+}
 
 // Rows, columns and phases as in k_rmsnorm; each thread keeps the weight gradient of its own
 // columns in registers over all its rows, and stores it four columns at a time (64 x 8192 BF16 10.6 us one
@@ -517,19 +797,14 @@ __global__ void __launch_bounds__(512) k_rmsnorm_grad(const NormGradParams p, in
 #pragma unroll
       for (int i = 0; i < NV; ++i) {
         if constexpr (!kKeep) w[0] = load_weight<WT, VE, SHIFT>(p.w, c, i);
-#pragma unroll
-        for (int j = 0; j < VE; ++j) {
-          const float d = elem<T>(dy.v[i], j), v = elem<T>(h.v[i], j);
-          a.sum = fmaf(d * elem<WT>(w[kKeep ? i : 0], j), v, a.sum);
-          dw[i][j] = fmaf(d * rstd, v, dw[i][j]);
-        }
+        grad_sums<T, WT, VE>(dy.v[i], h.v[i], w[kKeep ? i : 0], rstd, a.sum, dw[i]);
       }
       if constexpr (SHIFT) {
         a.sum = fmaf(dy.one * w1, h.one, a.sum);
         dw1 = fmaf(dy.one * rstd, h.one, dw1);
       }
     }
-    a = reduce_row(a, tpr, sm[half]);
+    a = reduce_row<false>(a, tpr, sm[half]);
     half ^= 1;
     if (live) {
       const float m = rstd * (a.sum * inv_cols);
@@ -538,13 +813,7 @@ __global__ void __launch_bounds__(512) k_rmsnorm_grad(const NormGradParams p, in
 #pragma unroll
       for (int i = 0; i < NV; ++i) {
         if constexpr (!kKeep) w[0] = load_weight<WT, VE, SHIFT>(p.w, c, i);
-        float o[VE];
-#pragma unroll
-        for (int j = 0; j < VE; ++j) {
-          o[j] = rstd * (elem<T>(dy.v[i], j) * elem<WT>(w[kKeep ? i : 0], j) - elem<T>(h.v[i], j) * rstd * m);
-          if (drs) o[j] += elem<T>(dr.v[i], j);
-        }
-        dy.v[i] = from_floats<T, VE>(o);
+        dy.v[i] = grad_output<T, WT, VE>(dy.v[i], h.v[i], w[kKeep ? i : 0], drs ? dr.v[i] : zero_words<sizeof(T) * VE>(), rstd, m);
       }
       if constexpr (SHIFT) {
         dy.one = rstd * (dy.one * w1 - h.one * rstd * m);
@@ -563,17 +832,7 @@ __global__ void __launch_bounds__(512) k_rmsnorm_grad(const NormGradParams p, in
   float* mine_out = tpr > 32 ? out : cols_sum + mine * p.cols;
 #pragma unroll
   for (int i = 0; i < NV; ++i)
-    if (c.has(i)) {
-      float* at = mine_out + c.col(i);
-      if (VE % 4 == 0 && (reinterpret_cast<uintptr_t>(at) & 15) == 0) {
-#pragma unroll
-        for (int j = 0; j + 3 < VE; j += 4)
-          *reinterpret_cast<float4*>(at + j) = make_float4(dw[i][j], dw[i][j + 1], dw[i][j + 2], dw[i][j + 3]);
-      } else {
-#pragma unroll
-        for (int j = 0; j < VE; ++j) at[j] = dw[i][j];
-      }
-    }
+    if (c.has(i)) store_sums<VE>(mine_out + c.col(i), dw[i]);
   if (SHIFT && c.single >= 0) mine_out[c.single] = dw1;
   if (tpr > 32) return;
   __syncthreads();
@@ -582,6 +841,114 @@ __global__ void __launch_bounds__(512) k_rmsnorm_grad(const NormGradParams p, in
     for (int g = 0; g < per_block; ++g) s += cols_sum[g * p.cols + j];
     out[j] = s;
   }
+}
+
+// k_rmsnorm_grad for many rows over 64 vectors: a block takes one row at a time out of its ring. In registers / staged, us, BF16
+// with a residual's gradient: 16384 x 8192 175 / 155, 23786 x 4608 195 / 129, 37476 x 3519 267 / 197, 6629 x 10184 166 / 108,
+// 31373 x 950 63 / 53; with few rows a block the first copies and barriers cost more than they save (1000 x 2050 FP32 11.1 / 12-18).
+template <typename T, typename WT, int VE, int NV, bool SHIFT>
+__global__ void __launch_bounds__(512) k_rmsnorm_grad_staged(const NormGradParams p) {
+  constexpr bool kKeep = kThreadBytes<T, VE, NV> <= 32;
+  extern __shared__ __align__(128) uint8_t ring_data[];
+  __shared__ uint64_t full[kMaxDepth];
+  __shared__ int abort_flag;
+  __shared__ SumMax sm[2][32];
+  const int tpr = blockDim.x, t = threadIdx.x;
+  const long long stride = gridDim.x;
+  long long row = blockIdx.x;
+  const Columns<VE, SHIFT> c(tpr, t, static_cast<int>((p.phase + row * p.ldh) & (VE - 1)), p.cols);
+  const T* dys = static_cast<const T*>(p.dy);
+  const T* hs = static_cast<const T*>(p.h);
+  const T* drs = static_cast<const T*>(p.dres);
+  RowRing<3> ring;
+  ring.full = full;
+  ring.data = ring_data;
+  ring.depth = p.depth;
+  ring.pitch = p.cols / VE * 16;
+  ring.src[0] = reinterpret_cast<const char*>(dys + row * p.lddy + c.front);
+  ring.src[1] = reinterpret_cast<const char*>(hs + row * p.ldh + c.front);
+  ring.src[2] = drs ? reinterpret_cast<const char*>(drs + row * p.lddr + c.front) : nullptr;
+  ring.step[0] = stride * p.lddy * sizeof(T);
+  ring.step[1] = stride * p.ldh * sizeof(T);
+  ring.step[2] = stride * p.lddr * sizeof(T);
+  ring.bytes = c.vecs * 16;
+  const WaitCtl wc{&abort_flag, p.status, p.budget_ns};
+  if (t == 0) {
+    for (int d = 0; d < p.depth; ++d) mbar_init(&full[d], 1);
+    abort_flag = 0;
+    fence_mbar_init();
+  }
+  grid_dependency_wait();
+  if (t == 0)
+    for (int d = 0; d < p.depth && row + d * stride < p.rows; ++d) ring.issue(d, d);
+  const float inv_cols = 1.f / static_cast<float>(p.cols);
+  Part<T, VE, NV, SHIFT> dy, h, dr;
+  Vec<WT, VE> w[kKeep ? NV : 1];
+  float dw[NV][VE], dw1 = 0.f, w1 = 0.f;
+  float rstd = 0.f, one_dy = 0.f, one_h = 0.f, one_dr = 0.f;
+  auto fetch_rest = [&](long long rw) {
+    if (rw >= p.rows) return;
+    rstd = p.rstd[rw];
+    if (!SHIFT || c.single < 0) return;
+    one_dy = to_f32(dys[rw * p.lddy + c.single]);
+    one_h = to_f32(hs[rw * p.ldh + c.single]);
+    if (drs) one_dr = to_f32(drs[rw * p.lddr + c.single]);
+  };
+  fetch_rest(row);
+  if constexpr (kKeep) {
+#pragma unroll
+    for (int i = 0; i < NV; ++i) w[i] = load_weight<WT, VE, SHIFT>(p.w, c, i);
+  }
+  if (SHIFT && c.single >= 0) w1 = to_f32(static_cast<const WT*>(p.w)[c.single]);
+#pragma unroll
+  for (int i = 0; i < NV; ++i)
+#pragma unroll
+    for (int j = 0; j < VE; ++j) dw[i][j] = 0.f;
+  __syncthreads();  // the barriers are set up
+  int half = 0;
+  for (long long n = 0; row < p.rows; ++n, row += stride) {
+    mbar_wait(&full[ring.slot], ring.parity, wc, 72);  // after a timeout the block goes on, with wrong values and the status set
+    load_staged(ring.at(ring.slot, 0), c, dy);
+    load_staged(ring.at(ring.slot, 1), c, h);
+    if (drs) load_staged(ring.at(ring.slot, 2), c, dr);
+    const float rs = rstd;
+    dy.one = one_dy;
+    h.one = one_h;
+    dr.one = one_dr;
+    fetch_rest(row + stride);
+    SumMax a{0.f, 0.f};
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      if constexpr (!kKeep) w[0] = load_weight<WT, VE, SHIFT>(p.w, c, i);
+      grad_sums<T, WT, VE>(dy.v[i], h.v[i], w[kKeep ? i : 0], rs, a.sum, dw[i]);
+    }
+    if constexpr (SHIFT) {
+      a.sum = fmaf(dy.one * w1, h.one, a.sum);
+      dw1 = fmaf(dy.one * rs, h.one, dw1);
+    }
+    __syncwarp();
+    a = reduce_row<false>(a, tpr, sm[half]);
+    half ^= 1;
+    // every thread has read its part of the slot
+    if (t == 0 && row + p.depth * stride < p.rows) ring.issue(ring.slot, n + p.depth);
+    ring.advance();
+    const float m = rs * (a.sum * inv_cols);
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      if constexpr (!kKeep) w[0] = load_weight<WT, VE, SHIFT>(p.w, c, i);
+      dy.v[i] = grad_output<T, WT, VE>(dy.v[i], h.v[i], w[kKeep ? i : 0], drs ? dr.v[i] : zero_words<sizeof(T) * VE>(), rs, m);
+    }
+    if constexpr (SHIFT) {
+      dy.one = rs * (dy.one * w1 - h.one * rs * m);
+      if (drs) dy.one += dr.one;
+    }
+    store_row(static_cast<T*>(p.dx) + row * p.lddx, c, dy);
+  }
+  float* out = p.partial + static_cast<long long>(blockIdx.x) * p.cols;
+#pragma unroll
+  for (int i = 0; i < NV; ++i)
+    if (c.has(i)) store_sums<VE>(out + c.col(i), dw[i]);
+  if (SHIFT && c.single >= 0) out[c.single] = dw1;
 }
 
 // Rows too long for registers: dx with the row read twice, and the weight gradient's slabs by
@@ -597,7 +964,7 @@ __global__ void __launch_bounds__(1024) k_rmsnorm_grad_wide(const NormGradParams
   const float rstd = p.rstd[row];
   SumMax a{0.f, 0.f};
   for (long long c = threadIdx.x; c < p.cols; c += 1024) a.sum = fmaf(to_f32(dy[c]) * to_f32(w[c]), to_f32(h[c]), a.sum);
-  a = reduce_row(a, 1024, sm);
+  a = reduce_row<false>(a, 1024, sm);
   const float m = rstd * (a.sum / static_cast<float>(p.cols));
   for (long long c = threadIdx.x; c < p.cols; c += 1024) {
     float g = rstd * (to_f32(dy[c]) * to_f32(w[c]) - to_f32(h[c]) * rstd * m);
@@ -712,11 +1079,77 @@ int launch_rows(const NormParams& p, const Shape& sh, cudaStream_t s, const Devi
   return BW_OK;
 }
 
+// A staged kernel's block (one row at a time, `want` vectors a thread or more), rows in flight and dynamic shared
+// memory, where an SM holds `resident` threads by their registers. depth = 0: the row is too long.
+struct Staging {
+  int nv, block, depth;
+  size_t smem;
+};
+constexpr int kRingBytes = 160 << 10, kRingMost = 200 << 10;  // of an SM; where two rows need more than the former
+Staging row_staging(long long nvec, int want, int max_nv, int tensors, int resident) {
+  Staging g{want, 0, 0, 0};
+  while (nvec > static_cast<long long>(g.nv) * kMaxThreads) g.nv *= 2;
+  if (nvec == 0 || g.nv > max_nv) return g;
+  g.block = static_cast<int>((nvec + 32 * g.nv - 1) / (32 * g.nv)) * 32;
+  const long long slot = tensors * nvec * 16;
+  int blocks = resident / g.block;
+  if (blocks < 1) blocks = 1;
+  while (blocks > 1 && kRingBytes / blocks < 2 * slot) --blocks;
+  long long depth = kRingBytes / blocks / slot;
+  if (depth < 2) depth = kRingMost / blocks / slot;
+  g.depth = static_cast<int>(depth > kMaxDepth ? kMaxDepth : depth);
+  g.smem = static_cast<size_t>(g.depth) * slot;
+  return g;
+}
+constexpr int kMaxDynamic = 225 << 10;
+
+// Blocks of a staged kernel that an SM holds.
+template <auto KERN>
+int staged_resident(const Staging& g, int* per_sm) {
+  static std::atomic<int> known[64][kMaxThreads / 32 + 1] = {};  // by device and block size, without the ring
+  int dev = 0;
+  BW_CUDA(cudaGetDevice(&dev));
+  std::atomic<int>& k = known[dev & 63][g.block / 32];
+  int n = k.load(std::memory_order_acquire);
+  if (n == 0) {
+    BW_CUDA(cudaFuncSetAttribute(KERN, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxDynamic));
+    BW_CUDA(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, KERN, g.block, 0));
+    k.store(n, std::memory_order_release);
+  }
+  const int fit = static_cast<int>((228u << 10) / (g.smem + 2048));  // 1 KB of the system's, 1 KB static
+  *per_sm = n < fit ? n : fit;
+  return BW_OK;
+}
+
+template <auto KERN, bool SHIFT>
+int launch_staged(NormParams p, const Staging& g, cudaStream_t s, const DeviceState& d) {
+  int per_sm = 0;
+  const int r = staged_resident<KERN>(g, &per_sm);
+  if (r != BW_OK) return r;
+  long long grid = static_cast<long long>(d.sms) * per_sm;
+  if (SHIFT) grid = grid / 8 * 8;
+  if (grid > p.rows) grid = p.rows;
+  p.depth = g.depth;
+  BW_CUDA(launch_dependent(KERN, dim3(static_cast<unsigned>(grid)), g.block, g.smem, s, p));
+  return BW_OK;
+}
+
 template <typename T, typename WT, bool Q8, int VE, bool SHIFT>
 int launch_norm(const NormParams& p, cudaStream_t s, const DeviceState& d) {
   constexpr int kMaxNv = VE == 1 ? 16 : sizeof(T) == 4 ? 8 : 4;
   const long long nvec = SHIFT ? p.cols / VE : (p.cols + VE - 1LL) / VE;
-  const Shape sh = row_shape(p.rows, nvec, 4, kMaxNv, SHIFT ? 16 : 1);
+  if constexpr (VE > 1) {
+    const Shape sh = row_shape(p.rows, nvec, 4, kMaxNv, 1);
+    // rows of whole vectors whose blocks leave few of an SM's 512 x 4 vectors unused
+    const bool full = !SHIFT && sh.nv == 4 && kMaxThreads / sh.block * nvec >= 1700;
+    if (nvec > 128 && p.rows * nvec > 148LL * 512 && !full) {
+      const Staging g = row_staging(nvec, 4, sizeof(T) == 4 ? 8 : 4, p.res ? 2 : 1, 768);
+      if (g.depth > 0 && g.nv == 4) return launch_staged<k_rmsnorm_staged<T, WT, Q8, VE, 4, SHIFT>, SHIFT>(p, g, s, d);
+      if constexpr (sizeof(T) == 4)
+        if (g.depth > 0) return launch_staged<k_rmsnorm_staged<T, WT, Q8, VE, 8, SHIFT>, SHIFT>(p, g, s, d);
+    }
+  }
+  const Shape sh = row_shape(p.rows, nvec, SHIFT && nvec <= 32 ? 1 : 4, kMaxNv, SHIFT ? 16 : 1);
   if (sh.nv == 0) {
     constexpr int WVE = SHIFT ? 1 : VE;
     BW_CUDA(launch_dependent(k_rmsnorm_wide<T, WT, Q8, WVE>, dim3(static_cast<unsigned>(p.rows)), 1024, 0, s, p));
@@ -813,6 +1246,9 @@ int norm_impl(const void* x, long long ldx, const void* residual, long long ldr,
   p.rows = rows;
   p.cols = cols;
   p.eps = eps;
+  p.inv_cols = 1.f / static_cast<float>(cols);
+  p.status = d->status;
+  p.budget_ns = wait_budget_ns();
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   if (dtype == BW_DTYPE_F32) return dispatch_weight<float>(p, q8, s, *d);
   if (dtype == BW_DTYPE_F16) return dispatch_weight<__half>(p, q8, s, *d);
@@ -821,19 +1257,54 @@ int norm_impl(const void* x, long long ldx, const void* residual, long long ldr,
 
 // Slabs of the weight gradient, one a block: a function of the sizes alone, so that the sums (and the
 // workspace) are the same on every device. 512 threads are resident on an SM (of 148) with this
-// kernel's registers, and a block has one for 16 columns, or 256 for short rows; more slabs wait for
-// those to end and write more partial sums (16384 x 8192 BF16: 180 us with 148, 185 with 296, 199 with 592).
+// kernel's registers (640 with the staged one's), and a block has one for 16 columns, or 256 for short rows; more
+// slabs wait for those to end (a whole second wave, 37476 x 3519 BF16: 267 us with 296, 411 with 338) and write more partial
+// sums (16384 x 8192 BF16: 180 us with 148, 199 with 592).
 int grad_slabs(long long rows, long long cols) {
   long long most = 296;
-  if (cols > 512 && cols <= 16384) most = 148LL * 512 / (cols > 8192 ? 512 : (cols + 511) / 512 * 32);
+  if (cols > 512 && cols <= 16384) {
+    const int threads = cols > 8192 ? 512 : static_cast<int>((cols + 511) / 512 * 32);
+    most = 148 * ((threads > 256 ? 640 : 512) / threads);
+  }
   if (cols <= 16384 && most > rows / 4) most = rows / 4 > 148 ? rows / 4 : 148;
   return static_cast<int>(rows < most ? rows : most);
+}
+
+int sum_slabs(const NormGradParams& p, float* dw, cudaStream_t s) {
+  BW_CUDA(launch_dependent(k_sum_slabs, dim3(static_cast<unsigned>((p.cols + 31LL) / 32)), 1024, 0, s,
+                           static_cast<const float*>(p.partial), dw, p.slabs, p.cols));
+  return BW_OK;
+}
+
+// A slab (block) for every row up to the workspace's slabs, and no more blocks than one wave of 148 SMs
+// holds by its ring and registers.
+template <auto KERN, bool SHIFT>
+int launch_grad_staged(NormGradParams p, const Staging& g, float* dw, cudaStream_t s) {
+  int per_sm = 0;
+  const int r = staged_resident<KERN>(g, &per_sm);
+  if (r != BW_OK) return r;
+  int most = 148 * per_sm;
+  if (most > p.slabs) most = p.slabs;
+  if (SHIFT && most > 8) most = most / 8 * 8;
+  p.slabs = p.rows < most ? static_cast<int>(p.rows) : most;
+  p.depth = g.depth;
+  BW_CUDA(launch_dependent(KERN, dim3(p.slabs), g.block, g.smem, s, p));
+  return sum_slabs(p, dw, s);
 }
 
 template <typename T, typename WT, int VE, bool SHIFT>
 int launch_grad(NormGradParams p, float* dw, cudaStream_t s) {
   constexpr int kMaxNv = VE == 1 ? 16 : sizeof(T) == 4 ? 8 : 4;
   const long long nvec = SHIFT ? p.cols / VE : (p.cols + VE - 1LL) / VE;
+  if constexpr (VE > 1) {
+    if (nvec > 64 && p.rows >= 8LL * p.slabs) {
+      constexpr int kNv = sizeof(T) == 4 ? 4 : 2;
+      const Staging g = row_staging(nvec, kNv, 4, p.dres ? 3 : 2, 512);
+      if (g.depth > 0 && g.nv == kNv) return launch_grad_staged<k_rmsnorm_grad_staged<T, WT, VE, kNv, SHIFT>, SHIFT>(p, g, dw, s);
+      if constexpr (kNv == 2)
+        if (g.depth > 0) return launch_grad_staged<k_rmsnorm_grad_staged<T, WT, VE, 4, SHIFT>, SHIFT>(p, g, dw, s);
+    }
+  }
   // 32 bytes of a row a thread (it fetches ahead then), 64 for long sums in FP32
   const Shape sh = row_shape(p.rows, nvec, sizeof(T) == 4 && p.rows >= 2048 ? 4 : 2, kMaxNv, SHIFT ? 16 : 1);
   if (sh.nv == 0) {
@@ -841,6 +1312,7 @@ int launch_grad(NormGradParams p, float* dw, cudaStream_t s) {
     BW_CUDA(launch_dependent(k_rmsnorm_dw_wide<T>, dim3(static_cast<unsigned>((p.cols + 255LL) / 256), p.slabs), 256, 0, s, p));
     BW_CUDA(launch_dependent(k_rmsnorm_grad_wide<T, WT>, dim3(static_cast<unsigned>(p.rows)), 1024, 0, s, p));
   } else {
+    if (sh.tpr > 32 && p.slabs > 148 * (kMaxThreads / sh.block)) p.slabs = 148 * (kMaxThreads / sh.block);
     const long long groups = (p.rows + sh.groups - 1) / sh.groups;
     if (groups <= p.slabs) p.slabs = static_cast<int>(groups);  // a row each
     else if (SHIFT && sh.groups < 8) p.slabs = p.slabs / 8 * 8;  // a stride of whole phases
@@ -858,9 +1330,7 @@ int launch_grad(NormGradParams p, float* dw, cudaStream_t s) {
         break;
     }
   }
-  BW_CUDA(launch_dependent(k_sum_slabs, dim3(static_cast<unsigned>((p.cols + 31LL) / 32)), 1024, 0, s,
-                           static_cast<const float*>(p.partial), dw, p.slabs, p.cols));
-  return BW_OK;
+  return sum_slabs(p, dw, s);
 }
 
 template <typename T, typename WT>
@@ -956,6 +1426,8 @@ int bw_rmsnorm_backward(const void* dy, long long lddy, const void* h, long long
   p.rows = rows;
   p.cols = cols;
   p.slabs = grad_slabs(rows, cols);
+  p.status = d->status;
+  p.budget_ns = wait_budget_ns();
   if (dtype == BW_DTYPE_F32) return dispatch_grad_weight<float>(p, dweight, s);
   if (dtype == BW_DTYPE_F16) return dispatch_grad_weight<__half>(p, dweight, s);
   return dispatch_grad_weight<__nv_bfloat16>(p, dweight, s);

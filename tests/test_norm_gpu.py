@@ -420,3 +420,99 @@ def test_large_offsets(cuda_dev):
     _check_forward(src, None, w, y, h, rstd)
     bwgemm.rmsnorm(x, w, eps=EPS, y=x)
     assert torch.equal(x, y)
+
+
+# rows enough that a block takes several, out of its shared memory: whole vectors or not, 2 to 16 warps a row,
+# one or more slots a block
+@pytest.mark.parametrize("rows,cols", [(1201, 1088), (1203, 1111), (700, 2498), (601, 4097), (333, 9553), (150, 16384),
+                                       (149, 16383), (2401, 520)])
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("residual", [False, True])
+def test_many_rows(cuda_dev, rows, cols, dtype, residual):
+    import torch
+
+    x, r, w = _inputs(cuda_dev, getattr(torch, dtype), rows, cols, residual, seed=rows + cols)
+    y, h, rstd = bwgemm.rmsnorm(x, w, residual=r, eps=EPS)
+    _check_forward(x, r, w, y, h, rstd)
+    q, s, h8, rstd8 = bwgemm.rmsnorm_fp8(x, w, residual=r, eps=EPS)
+    _check_fp8(x, r, w, q, s, h8, rstd8)
+    if residual:  # outputs over the inputs
+        xi, ri = x.clone(), r.clone()
+        yi, hi, rstdi = bwgemm.rmsnorm(xi, w, residual=ri, eps=EPS, y=xi, h=ri)
+        assert torch.equal(yi, y) and torch.equal(hi, h) and torch.equal(rstdi, rstd)
+    assert bwgemm.device_status() == 0
+
+
+@pytest.mark.parametrize("rows,cols", [(9601, 600), (9475, 1023), (2401, 4608), (2371, 4609), (1301, 9000), (1190, 16384),
+                                       (1185, 8191)])
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("dres", [False, True])
+def test_backward_many_rows(cuda_dev, rows, cols, dtype, dres):
+    import torch
+
+    dt = getattr(torch, dtype)
+    h, res, w = _inputs(cuda_dev, dt, rows, cols, dres, seed=rows + cols)
+    dy = torch.randn(rows, cols, device=cuda_dev).to(dt)
+    rstd = (h.double().square().mean(1) + EPS).rsqrt().float()
+    dx, dw = bwgemm.rmsnorm_backward(dy, h, w, rstd, dresidual=res)
+    _check_backward(dy, h, w, rstd, res, dx, dw)
+    again, dw2 = bwgemm.rmsnorm_backward(dy, h, w, rstd, dresidual=res)
+    assert torch.equal(dx, again) and torch.equal(dw, dw2)
+    over, dw3 = bwgemm.rmsnorm_backward(dy.clone(), h, w, rstd, dresidual=None if res is None else res, dx=h.clone())
+    assert torch.equal(over, dx) and torch.equal(dw3, dw)
+    own = dy.clone()
+    inplace, dw4 = bwgemm.rmsnorm_backward(own, h, w, rstd, dresidual=res, dx=own)
+    assert torch.equal(inplace, dx) and torch.equal(dw4, dw)
+    assert bwgemm.device_status() == 0
+
+
+def test_many_rows_of_a_pitch(cuda_dev):
+    """Rows inside wider buffers that start behind a vector's boundary, read through shared memory; what
+    lies around the outputs stays as it was."""
+    import torch
+
+    rows, cols, pad, shift = 1203, 1500, 13, 3
+    x, r, w = _inputs(cuda_dev, torch.bfloat16, rows, cols, True, seed=5)
+
+    def window(src, kind, fill):
+        whole = torch.full((rows * (cols + pad) + 64,), fill, dtype=kind, device=cuda_dev)
+        view = whole[shift:shift + rows * (cols + pad)].view(rows, cols + pad)[:, :cols]
+        if src is not None:
+            view.copy_(src)
+        return whole, view
+
+    xs, rs = window(x, x.dtype, 7.0)[1], window(r, x.dtype, 7.0)[1]
+    hw, h = window(None, x.dtype, 5.0)
+    qw, q = window(None, torch.uint8, 77)
+    q, s, h, rstd = bwgemm.rmsnorm_fp8(xs, w, residual=rs, eps=EPS, q=q, h=h)
+    _check_fp8(x, r, w, q.contiguous(), s, h, rstd)
+    h.fill_(5.0)
+    q.fill_(77)
+    assert bool((hw == 5.0).all()) and bool((qw == 77).all())
+
+
+def test_workspace_shared_by_captured_graphs(cuda_dev):
+    """Two graphs over one workspace, replayed one after the other on one stream."""
+    import torch
+
+    rows, cols = 2401, 4608
+    h, _, w = _inputs(cuda_dev, torch.bfloat16, rows, cols, False, seed=9)
+    rstd = (h.double().square().mean(1) + EPS).rsqrt().float()
+    dys = [torch.randn(rows, cols, device=cuda_dev).bfloat16() for _ in range(2)]
+    want = [bwgemm.rmsnorm_backward(dy, h, w, rstd) for dy in dys]
+    ws = torch.empty(bwgemm.rmsnorm_backward_workspace(rows, cols), dtype=torch.uint8, device=cuda_dev)
+    outs = [(torch.empty_like(h), torch.empty(cols, device=cuda_dev)) for _ in dys]
+    torch.cuda.synchronize()
+    stream = torch.cuda.Stream()
+    graphs = []
+    for dy, (dx, dw) in zip(dys, outs):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=stream):
+            bwgemm.rmsnorm_backward(dy, h, w, rstd, dx=dx, dweight=dw, workspace=ws)
+        graphs.append(graph)
+    for _ in range(3):
+        for graph in graphs:
+            graph.replay()
+    torch.cuda.synchronize()
+    for (dx, dw), (dx0, dw0) in zip(outs, want):
+        assert torch.equal(dx, dx0) and torch.equal(dw, dw0)
