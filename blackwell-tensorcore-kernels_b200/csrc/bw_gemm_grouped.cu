@@ -32,25 +32,11 @@ long long even_tile_rows(int rows, int groups, int tm) {
   return active * ((each + tm - 1) / tm);
 }
 
-// CTA pairs with 256 x 256 tiles where the groups have rows enough for them, and the tiles SMs enough:
-// measured against the single-CTA kernel over 32 groups of 2048 x 2048, E4M3 (BF16), by rows a group on
-// average: 96 35.6 / 35.3 us (62.3 / 60.7), 160 37.8 / 42.1 (64.9 / 74.2), 320 57.2 / 59.5, 640 86.8 / 96.4; weight gradient of
-// 1024 x 2048: 160 44.2 / 42.5, 224 49.4 / 51.0, 640 88.4 / 98.1. One group of 4096 x 4096 E4M3: 32 tiles (512
-// rows) 16.9 / 14.9 us, 64 tiles (1024 rows) 17.4 / 19.9.
-bool use_pair(const GroupedParams& p, bool wgrad, const DeviceState& d) {
-  const int forced = env_int("BW_GROUPED_PAIR", -1);
-  if (forced >= 0) return forced != 0;
-  const long long active = p.groups < p.rows ? p.groups : p.rows;
-  if (active == 0 || p.rows / active < (wgrad ? 192 : 144)) return false;
-  const long long tm = wgrad ? p.groups * ((p.m + 255LL) / 256) : even_tile_rows(p.rows, p.groups, 256);
-  return tm * ((p.n + 255LL) / 256) * 5 >= 2LL * d.sms;
-}
-
 // Tile width of the single-CTA kernel: the multiple of `gran` from 64 to 256 with the least work on the
 // busiest SM, ceil(tiles / SMs) x (W + c): a tile reads W columns of B and (in c) its rows of A, and
 // costs a start and an end. Ties go to the wider tile. 8 tokens' rows over 8 matrices of 4096 x 2048
 // E4M3: W = 240 (144 tiles, one wave).
-int tile_width(const GroupedParams& p, long long tile_rows, int gran, bool wgrad, const DeviceState& d) {
+int tile_width(const GroupedParams& p, long long tile_rows, int gran, bool wgrad, const DeviceState& d, long long* work = nullptr) {
   const int forced = env_int("BW_GROUPED_W", 0);
   if (forced >= 64 && forced <= 256 && forced % gran == 0) return forced;
   const long long active = p.groups < p.rows ? p.groups : p.rows;
@@ -66,7 +52,30 @@ int tile_width(const GroupedParams& p, long long tile_rows, int gran, bool wgrad
       W = w;
     }
   }
+  if (work) *work = best;
   return W;
+}
+
+// CTA pairs with 256 x 256 tiles where the groups have rows enough for them, and the tiles SMs enough:
+// measured against the single-CTA kernel over 32 groups of 2048 x 2048, E4M3 (BF16), by rows a group on
+// average: 96 35.6 / 35.3 us (62.3 / 60.7), 160 37.8 / 42.1 (64.9 / 74.2), 320 57.2 / 59.5, 640 86.8 / 96.4; weight gradient of
+// 1024 x 2048: 160 44.2 / 42.5, 224 49.4 / 51.0, 640 88.4 / 98.1, and of
+// 2008 x 2464, 60 groups of 187 213 / 234. One group of 4096 x 4096 E4M3: 32 tiles (512
+// rows) 16.9 / 14.9 us, 64 tiles (1024 rows) 17.4 / 19.9. A weight gradient of one or two rounds of pairs takes the kernel
+// with less work on the busiest SM, a pair's tile counting 354 on the scale of tile_width (256 + 160, less what it saves
+// in loads): 3 groups of 4005 rows, 3992 x 336 BF16 57.0 / 40.2 us.
+bool use_pair(const GroupedParams& p, bool wgrad, const DeviceState& d) {
+  const int forced = env_int("BW_GROUPED_PAIR", -1);
+  if (forced >= 0) return forced != 0;
+  const long long active = p.groups < p.rows ? p.groups : p.rows;
+  if (active == 0 || p.rows / active < (wgrad ? 160 : 144)) return false;
+  const long long tm = wgrad ? p.groups * ((p.m + 255LL) / 256) : even_tile_rows(p.rows, p.groups, 256);
+  const long long tiles = tm * ((p.n + 255LL) / 256), rounds = (2 * tiles + d.sms - 1) / d.sms;
+  if (tiles * 5 < 2LL * d.sms) return false;
+  if (!wgrad || rounds > 2) return true;
+  long long single;
+  tile_width(p, p.groups * ((p.m + 127LL) / 128), 64, true, d, &single);
+  return rounds * 354 <= single;
 }
 
 template <Kind KIND, GMode MODE, Out OUT>
