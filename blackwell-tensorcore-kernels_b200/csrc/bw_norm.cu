@@ -508,10 +508,12 @@ struct RowRing {
   const char* src[TENSORS];        // null: absent
   long long step[TENSORS];         // bytes between a block's rows
   uint32_t bytes;
+  int issued = 0;                  // rows, by the thread that issues them
 
   __device__ __forceinline__ int tensors() const { return src[TENSORS - 1] ? TENSORS : TENSORS - 1; }
   __device__ __forceinline__ uint8_t* at(int s, int tensor) const { return data + (s * tensors() + tensor) * pitch; }
-  __device__ __forceinline__ void issue(int s, long long n) const {  // the block's n-th row
+  __device__ __forceinline__ void issue(int s, long long n) {  // the block's n-th row
+    ++issued;
     mbar_arrive_expect_tx(&full[s], tensors() * bytes);
 #pragma unroll
     for (int i = 0; i < TENSORS; ++i)
@@ -519,6 +521,15 @@ struct RowRing {
   }
   __device__ __forceinline__ void advance() {
     if (++slot == depth) { slot = 0; parity ^= 1; }
+  }
+  // After a timeout the copies in flight land before the block gives its shared memory back.
+  __device__ __forceinline__ void drain(const WaitCtl& wc) const {
+    for (int i = issued > depth ? issued - depth : 0; i < issued; ++i) {
+      const uint64_t t0 = globaltimer_ns();
+      while (!mbar_try_wait(smem_u32(&full[i % depth]), static_cast<uint32_t>(i / depth) & 1u) &&
+             globaltimer_ns() - t0 < wc.budget_ns) {
+      }
+    }
   }
 };
 template <typename T, int VE, int NV, bool SHIFT>
@@ -537,7 +548,7 @@ __global__ void __launch_bounds__(512) k_rmsnorm_staged(const NormParams p) {
   constexpr bool kKeep = kThreadBytes<T, VE, NV> <= 64;
   extern __shared__ __align__(128) uint8_t ring_data[];
   __shared__ uint64_t full[kMaxDepth];
-  __shared__ int abort_flag;
+  __shared__ volatile int abort_flag;
   __shared__ SumMax sm[2][32];
   const int tpr = blockDim.x, t = threadIdx.x;
   const long long stride = gridDim.x;
@@ -610,7 +621,7 @@ __global__ void __launch_bounds__(512) k_rmsnorm_staged(const NormParams p) {
     a = reduce_row<Q8>(a, tpr, sm[half]);
     half ^= 1;
     // every thread has read its part of the slot
-    if (t == 0 && row + p.depth * stride < p.rows) ring.issue(ring.slot, n + p.depth);
+    if (t == 0 && row + p.depth * stride < p.rows && !abort_flag) ring.issue(ring.slot, n + p.depth);
     ring.advance();
     float pre;
     const float f = finish_row<Q8>(p, row, a, t == 0, pre);
@@ -623,6 +634,7 @@ __global__ void __launch_bounds__(512) k_rmsnorm_staged(const NormParams p) {
       if (c.single >= 0) store_words<sizeof(O)>(y + c.single, output<T, Q8, 1>(last, f, pre));
     }
   }
+  if (t == 0 && abort_flag) ring.drain(wc);
 }
 
 // Rows too long for the registers of one block: one block a row, which reads its row twice (the
@@ -844,14 +856,14 @@ __global__ void __launch_bounds__(512) k_rmsnorm_grad(const NormGradParams p, in
 }
 
 // k_rmsnorm_grad for many rows over 64 vectors: a block takes one row at a time out of its ring. In registers / staged, us, BF16
-// with a residual's gradient: 16384 x 8192 175 / 155, 23786 x 4608 195 / 129, 37476 x 3519 267 / 197, 6629 x 10184 166 / 108,
+// with a residual's gradient: 16384 x 8192 175 / 155, 23786 x 4608 195 / 129, 37476 x 3519 267 / 202, 6629 x 10184 166 / 104,
 // 31373 x 950 63 / 53; with few rows a block the first copies and barriers cost more than they save (1000 x 2050 FP32 11.1 / 12-18).
 template <typename T, typename WT, int VE, int NV, bool SHIFT>
 __global__ void __launch_bounds__(512) k_rmsnorm_grad_staged(const NormGradParams p) {
   constexpr bool kKeep = kThreadBytes<T, VE, NV> <= 32;
   extern __shared__ __align__(128) uint8_t ring_data[];
   __shared__ uint64_t full[kMaxDepth];
-  __shared__ int abort_flag;
+  __shared__ volatile int abort_flag;
   __shared__ SumMax sm[2][32];
   const int tpr = blockDim.x, t = threadIdx.x;
   const long long stride = gridDim.x;
@@ -930,7 +942,7 @@ __global__ void __launch_bounds__(512) k_rmsnorm_grad_staged(const NormGradParam
     a = reduce_row<false>(a, tpr, sm[half]);
     half ^= 1;
     // every thread has read its part of the slot
-    if (t == 0 && row + p.depth * stride < p.rows) ring.issue(ring.slot, n + p.depth);
+    if (t == 0 && row + p.depth * stride < p.rows && !abort_flag) ring.issue(ring.slot, n + p.depth);
     ring.advance();
     const float m = rs * (a.sum * inv_cols);
 #pragma unroll
@@ -944,6 +956,7 @@ __global__ void __launch_bounds__(512) k_rmsnorm_grad_staged(const NormGradParam
     }
     store_row(static_cast<T*>(p.dx) + row * p.lddx, c, dy);
   }
+  if (t == 0 && abort_flag) ring.drain(wc);
   float* out = p.partial + static_cast<long long>(blockIdx.x) * p.cols;
 #pragma unroll
   for (int i = 0; i < NV; ++i)
