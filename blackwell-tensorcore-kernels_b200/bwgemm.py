@@ -82,6 +82,7 @@ def lib():
         "bw_set_wait_budget_ns": [ctypes.c_ulonglong],
         "bw_set_trace_buffer": [P, I],
         "bw_selftest_bounded_wait": [ctypes.c_ulonglong, P],
+        "bw_selftest_grouped_wait": [I, I, P, P, P, I, P, I, I, I, I, I, I, ctypes.c_ulonglong, P, P],
         "bw_gemm_f16": [P, P, P, I, I, I, P],
         "bw_gemm_f16_bt": [P, P, P, I, I, I, P],
         "bw_gemm_fp8": [P, P, P, P, P, I, I, I, I, P],

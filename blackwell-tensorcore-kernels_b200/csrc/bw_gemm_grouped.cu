@@ -78,12 +78,13 @@ bool use_pair(const GroupedParams& p, bool wgrad, const DeviceState& d) {
   return rounds * 354 <= single;
 }
 
-template <Kind KIND, GMode MODE, Out OUT>
-int launch(const Operands& o, int dtype, GroupedParams p, cudaStream_t s, const DeviceState& d) {
+// STALL: the self-test of the waits, on the kernel that `pair_asked` names.
+template <Kind KIND, GMode MODE, Out OUT, bool STALL = false>
+int launch(const Operands& o, int dtype, GroupedParams p, cudaStream_t s, const DeviceState& d, bool pair_asked = false) {
   constexpr bool wgrad = MODE == GMode::WGRAD;
   constexpr int KE = KindTraits<KIND>::kElemsPerSlab;
   const int es = dtype == BW_DTYPE_FP8 ? 1 : 2;
-  const bool pair = use_pair(p, wgrad, d);
+  const bool pair = STALL ? pair_asked : use_pair(p, wgrad, d);
   const int tm = pair ? 256 : kBM;
   const long long mt = wgrad ? static_cast<long long>(p.groups) * ((p.m + tm - 1) / tm) : even_tile_rows(p.rows, p.groups, tm);
   p.W = pair ? 256 : tile_width(p, mt, MODE == GMode::ROWS_NK ? 16 : 64, wgrad, d);
@@ -117,8 +118,8 @@ int launch(const Operands& o, int dtype, GroupedParams p, cudaStream_t s, const 
   }
   int dev = 0;
   BW_CUDA(cudaGetDevice(&dev));
-  auto one = bw_tc_gemm_grouped_kernel<KIND, MODE, OUT>;
-  auto two = bw_tc_gemm_grouped_pair_kernel<KIND, MODE, OUT>;
+  auto one = bw_tc_gemm_grouped_kernel<KIND, MODE, OUT, STALL>;
+  auto two = bw_tc_gemm_grouped_pair_kernel<KIND, MODE, OUT, STALL>;
   static std::atomic<int> resident[64] = {};  // co-resident CTA pairs; 0: kernels not set up on this device
   int clusters = resident[dev & 63].load(std::memory_order_acquire);
   if (clusters == 0) {
@@ -246,6 +247,37 @@ int bw_gemm_grouped_wgrad(int dtype, const void* X, long long ldx, const void* Y
   p.n = N;
   const Operands o{X, Y, ldx, ldy};
   return launch_out<Kind::F16, GMode::WGRAD>(o, dtype, out_dtype, p, static_cast<cudaStream_t>(stream), *d);
+}
+
+int bw_selftest_grouped_wait(int pair, int wgrad, const void* A, const void* B, const int* offsets, int groups, void* C,
+                             int rows, int N, int K, int stall, int stop_leader, int stop_peer,
+                             unsigned long long budget_ns, int* landed, void* stream) {
+  const char* name = "self-test of the grouped products";
+  int r = check_grouped(name, BW_DTYPE_BF16, false, BW_OUT_BF16, offsets, groups, rows, N, K);
+  if (r != BW_OK) return r;
+  if (budget_ns == 0 || budget_ns > 1000000000ull) return set_error(BW_ERR_INVALID, "%s: budget must be in (0, 1 s]", name);
+  if (stall < 0 || stop_leader < 0 || stop_peer < 0) return set_error(BW_ERR_INVALID, "%s: negative slab", name);
+  if (rows == 0 || N == 0 || K == 0 || !C || !landed || !aligned16(C))
+    return set_error(BW_ERR_INVALID, "%s: empty size, or C or landed is null or not aligned", name);
+  if ((r = check_operand(name, "A", A, wgrad ? N : K, 2, wgrad ? N : K, 2)) != BW_OK || (r = check_operand(name, "B", B, K, 2, K, 2)) != BW_OK)
+    return r;
+  DeviceState* d;
+  if ((r = ensure_device(&d)) != BW_OK) return r;
+  GroupedParams p = base(*d, BW_DTYPE_BF16, C, wgrad ? K : N, BW_OUT_BF16, offsets, groups, rows);
+  (wgrad ? p.m : p.n) = N;
+  (wgrad ? p.n : p.k) = K;
+  p.budget_ns = budget_ns;
+  p.stall = stall;
+  p.stop[0] = stop_leader;
+  p.stop[1] = stop_peer;
+  p.landed = landed;
+  const Operands o{A, B, wgrad ? N : K, K};
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  r = wgrad ? launch<Kind::F16, GMode::WGRAD, Out::BF16, true>(o, BW_DTYPE_BF16, p, s, *d, pair != 0)
+            : launch<Kind::F16, GMode::ROWS_NK, Out::BF16, true>(o, BW_DTYPE_BF16, p, s, *d, pair != 0);
+  if (r != BW_OK) return r;
+  int st = 0;
+  return bw_device_status(stream, &st);
 }
 
 }  // extern "C"

@@ -46,6 +46,10 @@ struct GroupedParams {
   uint32_t fmt;              // operand format of the instruction descriptor
   int* status;
   unsigned long long budget_ns;
+  // self-test of the waits (instances with STALL only): the first CTA's (pair's) MMA thread waits for nothing in front of
+  // k-slab `stall`, its producers (leader, peer) take the wait in front of slab `stop` as timed out
+  int stall, stop[2];
+  int* landed;               // ... number of the CTA's stages whose last load was seen to land
 };
 
 // One lane of a converged warp. elect.sync (not a comparison of the lane index) tells the compiler
@@ -87,12 +91,10 @@ __device__ __forceinline__ bool mbar_wait_warp(uint64_t* bar, uint32_t parity, c
   return __all_sync(0xffffffffu, mbar_poll(bar, parity, w, where));
 }
 
-// Waits for a load of this CTA's own that is still in flight when a timeout ends the kernel early.
-__device__ __forceinline__ void mbar_drain(uint64_t* bar, uint32_t parity, uint64_t budget_ns) {
-  const uint32_t a = smem_u32(bar);
-  const uint64_t t0 = globaltimer_ns();
-  while (!mbar_try_wait(a, parity) && globaltimer_ns() - t0 < budget_ns) {
-  }
+// Takes `bytes` off what a barrier's current phase still expects.
+__device__ __forceinline__ void mbar_complete_tx(uint64_t* bar, uint32_t bytes) {
+  asm volatile("mbarrier.complete_tx.shared::cluster.relaxed.cluster.b64 [%0], %1;" ::"r"(smem_u32(bar)), "r"(bytes)
+               : "memory");
 }
 
 // bounds[g] = first row of group g (bounds[groups] = end of the last), clamped and made
@@ -302,9 +304,9 @@ __device__ __forceinline__ void grouped_epilogue(const GroupedParams& p, const G
 }
 
 __host__ __device__ constexpr int grouped_tail_bytes(int groups) {
-  // barriers (full, empty, tailfull, fixed per stage; accfull, accempty x 2; teardown), TMEM slot and abort
-  // flag, bounds and tiles, the epilogue's staging, alignment slack
-  return (4 * kGroupedMaxStages + 5) * 8 + 16 + 2 * (groups + 1) * 4 + kGroupedEpiWarps * kGroupedStageBytes + 1024;
+  // barriers (full, empty, tailfull, fixed per stage; accfull, accempty x 2; teardown), TMEM slot, abort flags and
+  // the pair's record of its loads, bounds and tiles, the epilogue's staging, alignment slack
+  return (4 * kGroupedMaxStages + 5) * 8 + 32 + 2 * (groups + 1) * 4 + kGroupedEpiWarps * kGroupedStageBytes + 1024;
 }
 
 // A tile of few rows loads them in boxes of 16 (a box of 128 rows would fetch its neighbours' too, and
@@ -332,7 +334,7 @@ __device__ __forceinline__ bool slab_is_cut(int left, int slab) { return left < 
 // other half of Tensor Memory. A tile has 128 rows however few count: their products cost nothing while the weights
 // arrive, and narrower tiles would read them again.
 // One CTA a tile of 128 x W (W <= 256; a multiple of 16, for an N-contiguous B of 64).
-template <Kind KIND, GMode MODE, Out OUT>
+template <Kind KIND, GMode MODE, Out OUT, bool STALL = false>
 __global__ void __launch_bounds__(kGroupedThreads, 1)
     bw_tc_gemm_grouped_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmA16,
                               const __grid_constant__ CUtensorMap tmB, const GroupedParams p) {
@@ -405,6 +407,7 @@ __global__ void __launch_bounds__(kGroupedThreads, 1)
         const int nk = (o.k + KE - 1) / KE;
         const uint64_t pol_b = o.b_once ? pol_once : pol_more;
         for (int kb = 0; kb < nk; ++kb) {
+          if (STALL && blockIdx.x == 0 && issued == p.stop[0]) { ok = false; break; }
           if (!mbar_poll(&empty[s], ph ^ 1, wc, 21)) { ok = false; break; }
           uint8_t* sA = smem + static_cast<size_t>(s) * p.stage_bytes;
           uint8_t* sB = sA + p.sub * kABytes;
@@ -452,12 +455,14 @@ __global__ void __launch_bounds__(kGroupedThreads, 1)
           if (++s == S) { s = 0; ph ^= 1; }
         }
       }
-      if (!ok)  // a timeout: loads in flight must land before the CTA gives its shared memory back
-        for (long long i = issued > S ? issued - S : 0; i < issued; ++i) {
-          const int st = static_cast<int>(i % S);
-          if ((cut_last >> st) & 1u) mbar_drain(&tailfull[st], ((cut_ph >> st) & 1u) ^ 1u, p.budget_ns);
-          else mbar_drain(&full[st], static_cast<uint32_t>(i / S) & 1u, p.budget_ns);
-        }
+      // Every load lands before the CTA gives its shared memory back, whichever thread's wait may have
+      // timed out: this one has issued its last slabs long before the others are done with them.
+      for (int i = 0; i < S && i < issued; ++i) {
+        if (--s < 0) { s = S - 1; ph ^= 1; }
+        const bool cut = (cut_last >> s) & 1u;
+        const bool in = mbar_drain(cut ? &tailfull[s] : &full[s], cut ? ((cut_ph >> s) & 1u) ^ 1u : ph);
+        if (STALL && blockIdx.x == 0 && in) atomicAdd(p.landed, 1);
+      }
     }
   } else if (warp == 1) {
     // ---------------- MMA issuer ----------------
@@ -467,6 +472,7 @@ __global__ void __launch_bounds__(kGroupedThreads, 1)
       uint32_t ph = 0, fixed_ph = 0;  // fixed_ph: one parity bit a stage
       int local = 0;
       bool ok = true;
+      [[maybe_unused]] int slab = 0;
       for (int t = blockIdx.x; t < num_tiles && ok; t += gridDim.x) {
         const GTile o = walk.at(t);
         const int nk = (o.k + KE - 1) / KE;
@@ -478,6 +484,8 @@ __global__ void __launch_bounds__(kGroupedThreads, 1)
         tc_fence_after();
         const uint32_t d_tmem = tmem_base + b * 256;
         for (int kb = 0; kb < nk; ++kb) {
+          if constexpr (STALL)
+            if (blockIdx.x == 0 && slab++ == p.stall && !mbar_poll(teardown, 0, wc, 27)) { ok = false; break; }
           if (!mbar_poll(&full[s], ph, wc, 23)) { ok = false; break; }
           const int left = o.k - kb * KE;
           // WGRAD: k-steps with rows of the group; else whole atoms (zeros behind K)
@@ -507,7 +515,7 @@ __global__ void __launch_bounds__(kGroupedThreads, 1)
         if (ok) umma_commit(&accfull[b]);
       }
       umma_commit(teardown);
-      mbar_drain(teardown, 0, p.budget_ns);
+      mbar_drain(teardown, 0);
     }
   } else if (warp < 2 + kGroupedEpiWarps) {
     // ---------------- epilogue ----------------
@@ -608,7 +616,7 @@ __device__ __forceinline__ bool mbar_wait_cluster(uint64_t* bar, uint32_t parity
   }
 }
 
-template <Kind KIND, GMode MODE, Out OUT>
+template <Kind KIND, GMode MODE, Out OUT, bool STALL = false>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGroupedThreads, 1)
     bw_tc_gemm_grouped_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmA16,
                                    const __grid_constant__ CUtensorMap tmB, const GroupedParams p) {
@@ -630,7 +638,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGroupedThreads, 1)
   uint64_t* teardown = accempty + 2;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(teardown + 1);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
-  int* bounds = reinterpret_cast<int*>(tmem_slot + 4);
+  volatile int* peer_abort = reinterpret_cast<volatile int*>(tmem_slot + 2);  // the other CTA's abort flag, written at the end
+  uint32_t* loads = tmem_slot + 3;  // what this CTA's producer leaves: slabs issued, bytes of `peer_units`
+  int* bounds = reinterpret_cast<int*>(tmem_slot + 8);
   int* tiles = bounds + p.groups + 1;
 
   const int warp = threadIdx.x >> 5;
@@ -650,6 +660,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGroupedThreads, 1)
     for (int b = 0; b < 2; ++b) { mbar_init(&accfull[b], 1); mbar_init(&accempty[b], 2 * kGroupedEpiWarps); }
     mbar_init(teardown, 1);
     *abort_flag = 0;
+    *peer_abort = 0;
     fence_mbar_init();
   }
   if (warp == 0 && lane == 0 && (MODE == GMode::WGRAD ? p.rows : p.k) > 0) { tma_prefetch_desc(&tmA); tma_prefetch_desc(&tmB); }
@@ -673,7 +684,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGroupedThreads, 1)
       const uint32_t full_leader = mapa_shared(smem_u32(full), 0);
       int s = 0;
       uint32_t ph = 0;
-      long long issued = 0;
+      uint32_t issued = 0;
+      uint32_t peer_units = 0;  // a byte a stage: what the peer's loads of its last slab add to full, in units of 2 KB
       uint32_t cut_last = 0, cut_ph = 0;
       bool ok = true;
       for (int t = cluster; t < num_tiles && ok; t += nclusters) {
@@ -681,17 +693,22 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGroupedThreads, 1)
         const int nk = (o.k + KE - 1) / KE;
         const int arow = o.row0 + half, bcol = o.col0 + half;
         const int valid = min(128, o.rows - half);  // ROWS: this CTA's rows of the tile (may be <= 0)
-        const uint32_t a_bytes = a_load_bytes(min(128, o.rows)) + (o.rows > 128 ? a_load_bytes(o.rows - 128) : 0);
+        const uint32_t peer_a = o.rows > 128 ? a_load_bytes(o.rows - 128) : 0;
+        const uint32_t a_bytes = a_load_bytes(min(128, o.rows)) + peer_a;
         for (int kb = 0; kb < nk; ++kb) {
+          if (STALL && cluster == 0 && issued == static_cast<uint32_t>(p.stop[rank])) { ok = false; break; }
           if (!mbar_poll(&empty[s], ph ^ 1, wc, 61)) { ok = false; break; }
           uint8_t* sA = smem + s * kPairStageBytes;
           uint8_t* sB = sA + kPairSub * kPairAtom;
           uint32_t bar = full_leader + s * 8;
           const int left = o.k - kb * KE;
           const int atoms = left > KA ? 2 : 1;
+          const bool cut = A_MN && slab_is_cut(left, KE);
+          const uint32_t units = cut ? 0u : atoms * (A_MN ? 2 * kPairAtom : peer_a + kPairAtom) / 2048;
+          peer_units = (peer_units & ~(255u << (8 * s))) | units << (8 * s);
           if constexpr (A_MN) {
             // a cut slab's two halves land on barriers of their own CTA's (see the single-CTA kernel)
-            if (slab_is_cut(left, KE)) {
+            if (cut) {
               if (leader) mbar_arrive(&full[s]);
               bar = smem_u32(&tailfull[s]);
               mbar_arrive_expect_tx(&tailfull[s], atoms * 2 * kPairAtom);
@@ -731,12 +748,15 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGroupedThreads, 1)
           if (++s == S) { s = 0; ph ^= 1; }
         }
       }
-      if (!ok)  // a timeout: loads in flight land before the CTAs end (the leader counts both CTAs' on full)
-        for (long long i = issued > S ? issued - S : 0; i < issued; ++i) {
-          const int st = static_cast<int>(i % S);
-          if ((cut_last >> st) & 1u) mbar_drain(&tailfull[st], ((cut_ph >> st) & 1u) ^ 1u, p.budget_ns);
-          else if (leader) mbar_drain(&full[st], static_cast<uint32_t>(i / S) & 1u, p.budget_ns);
+      // cut slabs land on barriers of this CTA's own; the others are waited for at the end, where it is known
+      // whether both CTAs issued them
+      for (int st = 0; st < S; ++st)
+        if ((cut_last >> st) & 1u) {
+          const bool in = mbar_drain(&tailfull[st], ((cut_ph >> st) & 1u) ^ 1u);
+          if (STALL && cluster == 0 && in) atomicAdd(p.landed, 1);
         }
+      loads[0] = issued;
+      loads[1] = peer_units;
     }
   } else if (warp == 1) {
     // ---------------- MMA issuer (leader CTA only) ----------------
@@ -748,6 +768,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGroupedThreads, 1)
       uint32_t ph = 0, fixed_ph = 0;
       int local = 0;
       bool ok = true;
+      [[maybe_unused]] int slab = 0;
       for (int t = cluster; t < num_tiles && ok; t += nclusters) {
         const GTile o = walk.at(t);
         const int nk = (o.k + KE - 1) / KE;
@@ -759,6 +780,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGroupedThreads, 1)
         tc_fence_after();
         const uint32_t d_tmem = tmem_base + b * 256;
         for (int kb = 0; kb < nk; ++kb) {
+          if constexpr (STALL)
+            if (cluster == 0 && slab++ == p.stall && !mbar_poll(teardown, 0, wc, 67)) { ok = false; break; }
           if (!mbar_poll(&full[s], ph, wc, 63)) { ok = false; break; }
           const int left = o.k - kb * KE;
           // WGRAD: k-steps with rows of the group; else whole atoms (zeros behind K)
@@ -798,7 +821,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGroupedThreads, 1)
         }
       }
       umma_commit_pair(smem_u32(teardown));
-      mbar_drain(teardown, 0, p.budget_ns);
+      mbar_drain(teardown, 0);
     }
   } else if (warp < 2 + kGroupedEpiWarps) {
     // ---------------- epilogue (both CTAs) ----------------
@@ -854,7 +877,29 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGroupedThreads, 1)
 
   tc_fence_before();
   __syncthreads();
+  if (threadIdx.x == 0 && *abort_flag) st_shared_cluster(mapa_shared(smem_u32(const_cast<int*>(peer_abort)), rank ^ 1), 1);
+  __syncwarp();
   cluster_sync();
+  if (*abort_flag || *peer_abort) {
+    // A wait timed out in one of the CTAs: both come here. The loads of both land before either ends. They are counted on
+    // the leader's full[s], which expects a slab's bytes from both CTAs as soon as the leader issues its half; where only one
+    // has issued the stage's last slab, the phase is made to expect that one's bytes alone. (The two are
+    // at most a slab a stage apart: the MMA thread frees no stage that lacks a half.)
+    if (leader && threadIdx.x == 0) {
+      const uint32_t theirs = mapa_shared(smem_u32(loads), 1);
+      const uint32_t n0 = loads[0], n1 = ld_shared_cluster(theirs), units0 = loads[1], units1 = ld_shared_cluster(theirs + 4);
+      for (int s = 0; s < S; ++s) {
+        const uint32_t u0 = (n0 + S - 1 - s) / S, u1 = (n1 + S - 1 - s) / S;  // times that the stage was filled
+        if (u1 > u0) mbar_arrive_expect_tx(&full[s], ((units1 >> (8 * s)) & 255u) * 2048);
+        else if (u0 > u1 && ((units0 >> (8 * s)) & 255u)) mbar_complete_tx(&full[s], ((units0 >> (8 * s)) & 255u) * 2048);
+        const uint32_t u = max(u0, u1);
+        const bool in = u == 0 || mbar_drain(&full[s], (u - 1) & 1u);
+        if (STALL && cluster == 0 && u > 0 && in) atomicAdd(p.landed, 256);
+      }
+    }
+    __syncthreads();
+    cluster_sync();
+  }
   if (warp == 1) {
     __syncwarp();
     tc_fence_after();

@@ -91,6 +91,20 @@ __device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity, const 
   }
 }
 
+// Waits for work of this CTA's own that is still in flight when its threads are done: loads into its
+// shared memory, MMAs on its Tensor Memory. They end by themselves within microseconds, so the limit
+// has nothing to do with the wait budget (which a caller may set to anything). True: the phase is over.
+constexpr uint64_t kDrainNs = 1000000000ull;
+__device__ __forceinline__ bool mbar_drain(uint64_t* bar, uint32_t parity) {
+  const uint32_t a = smem_u32(bar);
+  if (mbar_try_wait(a, parity)) return true;
+  const uint64_t t0 = globaltimer_ns();
+  do {
+    if (mbar_try_wait(a, parity)) return true;
+  } while (globaltimer_ns() - t0 < kDrainNs);
+  return false;
+}
+
 // ------------------------------------------------------------------------------------
 // TMA (cp.async.bulk.tensor), tiled, no multicast. Completion is counted on an mbarrier.
 // ------------------------------------------------------------------------------------
@@ -272,6 +286,14 @@ __device__ __forceinline__ uint32_t mapa_shared(uint32_t saddr, uint32_t rank) {
   uint32_t r;
   asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(saddr), "r"(rank));
   return r;
+}
+__device__ __forceinline__ void st_shared_cluster(uint32_t cluster_addr, uint32_t v) {
+  asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(cluster_addr), "r"(v) : "memory");
+}
+__device__ __forceinline__ uint32_t ld_shared_cluster(uint32_t cluster_addr) {
+  uint32_t v;
+  asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(cluster_addr) : "memory");
+  return v;
 }
 __device__ __forceinline__ void mbar_arrive_cluster(uint32_t cluster_addr) {
   asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");

@@ -84,6 +84,16 @@ int bw_set_trace_buffer(unsigned long long* dev_buf, int max_ctas);
  * wait as the GEMM kernels; returns BW_ERR_TIMEOUT after about budget_ns with the device
  * status word cleared again, leaving the context usable. */
 int bw_selftest_bounded_wait(unsigned long long budget_ns, void* stream);
+/* The same for the grouped products: the first CTA (pair = 0) or CTA pair of a BF16 launch gives up in the middle, and
+ * every load that it issued has to land before it ends. Its MMA thread waits for nothing in front of k-slab `stall`; its producer
+ * (of a pair: the leader's, the peer's) takes the wait in front of slab stop_leader, stop_peer as timed out; a number
+ * behind its last slab: not at all. wgrad = 0: A rows x K, B groups x N x K, C rows x N; wgrad = 1: A rows x N, B rows x K,
+ * C groups x N x K; all BF16 and contiguous, sizes as in bw_gemm_grouped. budget_ns: of each wait, up to 1 s. *landed (device memory)
+ * is increased by what was seen to land: single CTA, 1 a pipeline stage with a load in it; pair, 256 a stage, and 1 for each
+ * CTA's last slab of a stage that ends inside a k-step (wgrad). Returns BW_ERR_TIMEOUT with the status word cleared. */
+int bw_selftest_grouped_wait(int pair, int wgrad, const void* A, const void* B, const int* offsets, int groups, void* C,
+                             int rows, int N, int K, int stall, int stop_leader, int stop_peer,
+                             unsigned long long budget_ns, int* landed, void* stream);
 /* Overrides the per-wait budget of every kernel (nanoseconds; default 2e9). */
 int bw_set_wait_budget_ns(unsigned long long ns);
 
