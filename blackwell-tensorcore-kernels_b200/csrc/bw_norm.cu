@@ -522,14 +522,11 @@ struct RowRing {
   __device__ __forceinline__ void advance() {
     if (++slot == depth) { slot = 0; parity ^= 1; }
   }
-  // After a timeout the copies in flight land before the block gives its shared memory back.
-  __device__ __forceinline__ void drain(const WaitCtl& wc) const {
-    for (int i = issued > depth ? issued - depth : 0; i < issued; ++i) {
-      const uint64_t t0 = globaltimer_ns();
-      while (!mbar_try_wait(smem_u32(&full[i % depth]), static_cast<uint32_t>(i / depth) & 1u) &&
-             globaltimer_ns() - t0 < wc.budget_ns) {
-      }
-    }
+  // After a timeout the copies in flight land before the block gives its shared memory back, however
+  // short the wait budget is.
+  __device__ __forceinline__ void drain() const {
+    for (int i = issued > depth ? issued - depth : 0; i < issued; ++i)
+      mbar_drain(&full[i % depth], static_cast<uint32_t>(i / depth) & 1u);
   }
 };
 template <typename T, int VE, int NV, bool SHIFT>
@@ -634,7 +631,7 @@ __global__ void __launch_bounds__(512) k_rmsnorm_staged(const NormParams p) {
       if (c.single >= 0) store_words<sizeof(O)>(y + c.single, output<T, Q8, 1>(last, f, pre));
     }
   }
-  if (t == 0 && abort_flag) ring.drain(wc);
+  if (t == 0 && abort_flag) ring.drain();
 }
 
 // Rows too long for the registers of one block: one block a row, which reads its row twice (the
@@ -956,7 +953,7 @@ __global__ void __launch_bounds__(512) k_rmsnorm_grad_staged(const NormGradParam
     }
     store_row(static_cast<T*>(p.dx) + row * p.lddx, c, dy);
   }
-  if (t == 0 && abort_flag) ring.drain(wc);
+  if (t == 0 && abort_flag) ring.drain();
   float* out = p.partial + static_cast<long long>(blockIdx.x) * p.cols;
 #pragma unroll
   for (int i = 0; i < NV; ++i)
