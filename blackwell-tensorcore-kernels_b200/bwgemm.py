@@ -408,7 +408,8 @@ def rmsnorm(x, weight, residual=None, eps: float = 1e-6, y=None, h=None, rstd=No
 
     x, residual, y, h: rows x cols of float32, float16 or bfloat16 with contiguous rows; weight of
     the same type or float32. h (x itself where there is no residual) and rstd are what
-    rmsnorm_backward takes. y and h may be x's or the residual's own tensor."""
+    rmsnorm_backward takes. y and h may each be x's or the residual's own tensor, not both the same one.
+    Where y is written over x without a residual, x no longer holds h: the h returned is None unless one is given."""
     import torch
 
     code, wcode, dtype, shape, dev, ldx, ldr = _norm_operands(x, weight, residual)
@@ -422,6 +423,8 @@ def rmsnorm(x, weight, residual=None, eps: float = 1e-6, y=None, h=None, rstd=No
         _check(lib().bw_rmsnorm(x.data_ptr(), ldx, _ptr(residual), ldr, weight.data_ptr(), code, wcode, eps,
                                 y.data_ptr(), ldy, _ptr(hout), ldh, rstd.data_ptr(), shape[0], shape[1],
                                 _current_stream(dev)))
+    if h is x and hout is None and y.data_ptr() == x.data_ptr():
+        h = None
     return y, h, rstd
 
 

@@ -1210,6 +1210,13 @@ int check_ptr(const char* what, const void* p, int align) {
   return BW_OK;
 }
 
+// An output over an input: row by row, so both need one pitch.
+int check_in_place(const char* out, const void* o, long long ldo, const char* in, const void* i, long long ldi, int rows) {
+  if (o && o == i && rows > 1 && ldo != ldi)
+    return set_error(BW_ERR_INVALID, "%s over %s: row pitches %lld and %lld differ", out, in, ldo, ldi);
+  return BW_OK;
+}
+
 int check_norm_common(int dtype, int weight_dtype, int rows, int cols) {
   if (!norm_dtype_ok(dtype)) return set_error(BW_ERR_INVALID, "rmsnorm takes F32, F16 or BF16 (dtype %d)", dtype);
   if (weight_dtype != dtype && weight_dtype != BW_DTYPE_F32)
@@ -1238,6 +1245,13 @@ int norm_impl(const void* x, long long ldx, const void* residual, long long ldr,
     return r;
   if (residual && (r = check_pitch("residual", ldr, rows, cols)) != BW_OK) return r;
   if (h && (r = check_pitch("h", ldh, rows, cols)) != BW_OK) return r;
+  if (y == h) return set_error(BW_ERR_INVALID, "%s and h are one buffer", q8 ? "q" : "y");
+  if (q8 && (y == x || y == residual)) return set_error(BW_ERR_INVALID, "q over an input: elements of different size");
+  if ((r = check_in_place("y", y, ldy, "x", x, ldx, rows)) != BW_OK ||
+      (r = check_in_place("y", y, ldy, "residual", residual, ldr, rows)) != BW_OK ||
+      (r = check_in_place("h", h, ldh, "x", x, ldx, rows)) != BW_OK ||
+      (r = check_in_place("h", h, ldh, "residual", residual, ldr, rows)) != BW_OK)
+    return r;
   DeviceState* d;
   if ((r = ensure_device(&d)) != BW_OK) return r;
   NormParams p{};
@@ -1416,6 +1430,10 @@ int bw_rmsnorm_backward(const void* dy, long long lddy, const void* h, long long
       (r = check_pitch("dx", lddx, rows, cols)) != BW_OK)
     return r;
   if (dresidual && (r = check_pitch("dresidual", lddr, rows, cols)) != BW_OK) return r;
+  if ((r = check_in_place("dx", dx, lddx, "dy", dy, lddy, rows)) != BW_OK ||
+      (r = check_in_place("dx", dx, lddx, "h", h, ldh, rows)) != BW_OK ||
+      (r = check_in_place("dx", dx, lddx, "dresidual", dresidual, lddr, rows)) != BW_OK)
+    return r;
   const size_t need = bw_rmsnorm_backward_workspace(rows, cols);
   if (workspace_bytes < need)
     return set_error(BW_ERR_INVALID, "workspace holds %zu bytes, rmsnorm backward needs %zu", workspace_bytes, need);

@@ -172,8 +172,9 @@ size_t bw_sf_offset(int row, int kblock, int K);
  * small that 448 / amax overflows), q = cvt(y * (448 / amax)), satfinite.
  * dtype: BW_DTYPE_F32, F16 or BF16 (x, residual, y, h); weight_dtype: the same or BW_DTYPE_F32.
  * h and rstd may be NULL (not wanted). ld*: row pitches in elements, at least cols. Any alignment
- * to whole elements; 16-byte aligned rows run faster. y and h may be x's or the residual's own
- * buffer (same type, same pitch); other overlap is not allowed. Sums are FP32: a row whose squares
+ * to whole elements; 16-byte aligned rows run faster. y and h may each be x's or the residual's own
+ * buffer (same type, same pitch), not both the same one; other overlap is not allowed. With y over x and no
+ * residual, the h that the gradient needs is gone unless it is asked for. Sums are FP32: a row whose squares
  * sum to more than FP32 holds gets rstd = 0, one with a NaN, or of zeros with eps = 0, gets NaN (codes
  * 0x7f, scale 1). */
 int bw_rmsnorm(const void* x, long long ldx, const void* residual, long long ldr, const void* weight, int dtype,
