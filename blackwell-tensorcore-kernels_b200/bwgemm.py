@@ -317,6 +317,13 @@ def _dtype_code(t, what: str, allowed: tuple[int, ...]) -> int:
     return code
 
 
+_INT_MAX = 2 ** 31 - 1  # ctypes would pass on the low 32 bits of more
+
+
+def _too_large(*sizes):
+    raise ValueError(f"a size of {max(sizes)} exceeds {_INT_MAX}")
+
+
 def _refuse(what: str, t, shape, dtype, dev: int):
     if t.dtype != dtype:
         raise TypeError(f"{what} must be {dtype}, not {t.dtype}")
@@ -377,6 +384,8 @@ def _norm_operands(x, weight, residual):
     if x.dim() != 2 or weight.dim() != 1:
         raise ValueError(f"rmsnorm takes x (rows x cols) and weight (cols), not {x.dim()}-D and {weight.dim()}-D")
     dtype, shape, dev = x.dtype, x.shape, x.get_device()
+    if shape[0] > _INT_MAX or shape[1] > _INT_MAX:
+        _too_large(*shape)
     code = _dtype_code(x, "x", _NORM_TYPES)
     wtype = weight.dtype
     if wtype is not dtype and _codes().get(wtype) != DTYPE_F32:
@@ -454,6 +463,8 @@ def rmsnorm_fp8(x, weight, residual=None, eps: float = 1e-6, q=None, row_scale=N
 @functools.lru_cache(maxsize=256)
 def rmsnorm_backward_workspace(rows: int, cols: int) -> int:
     """Bytes of workspace that rmsnorm_backward needs for these sizes."""
+    if rows > _INT_MAX or cols > _INT_MAX:
+        _too_large(rows, cols)
     return int(lib().bw_rmsnorm_backward_workspace(rows, cols))
 
 
@@ -506,6 +517,8 @@ def _groups(offsets, dev: int) -> int:
 
     if offsets.dim() != 1 or offsets.shape[0] < 2:
         raise ValueError(f"offsets must hold groups + 1 ints, not a tensor of shape {tuple(offsets.shape)}")
+    if offsets.shape[0] > _INT_MAX:
+        _too_large(offsets.shape[0])
     _flat("offsets", offsets, offsets.shape, torch.int32, dev)
     return offsets.shape[0] - 1
 
@@ -525,6 +538,8 @@ def gemm_grouped(A, B, offsets, C=None, b_transposed: bool = False, row_scale=No
     code = _dtype_code(A, "A", (DTYPE_F16, DTYPE_BF16, DTYPE_FP8))
     (rows, K), dev = A.shape, A.get_device()
     N = B.shape[1] if b_transposed else B.shape[2]
+    if rows > _INT_MAX or K > _INT_MAX or N > _INT_MAX:
+        _too_large(rows, K, N)
     groups = _groups(offsets, dev)
     _flat("B", B, (groups, N, K) if b_transposed else (groups, K, N), A.dtype, dev)
     lda = _rows("A", A, A.shape, A.dtype, dev)
@@ -555,6 +570,8 @@ def gemm_grouped_wgrad(X, Y, offsets, D=None, out_dtype=OUT_F32, stream=None):
         raise ValueError(f"gemm_grouped_wgrad takes X (rows x M) and Y (rows x N), not {X.dim()}-D and {Y.dim()}-D")
     code = _dtype_code(X, "X", (DTYPE_F16, DTYPE_BF16))
     (rows, M), N, dev = X.shape, Y.shape[1], X.get_device()
+    if rows > _INT_MAX or M > _INT_MAX or N > _INT_MAX:
+        _too_large(rows, M, N)
     groups = _groups(offsets, dev)
     ldx = _rows("X", X, X.shape, X.dtype, dev)
     ldy = _rows("Y", Y, (rows, N), X.dtype, dev)
