@@ -224,35 +224,49 @@ __device__ __forceinline__ void grouped_epilogue(const GroupedParams& p, const G
     return;
   }
   const int nrows = min(32, t.rows - first);
-  long long row;
-  float alpha = 1.f;
-  if constexpr (MODE == GMode::WGRAD) {
-    row = static_cast<long long>(t.g) * p.m + t.row0 + first;
-  } else {
-    row = t.row0 + first;
-    if (t.k > 0) {
-      if (p.group_scale) alpha *= __ldcg(p.group_scale + t.g);
-      if (p.row_scale && lane < nrows) alpha *= __ldcg(p.row_scale + row + lane);
-    }
-  }
-  const long long pitch = p.ldc * kElem;
-  char* out = static_cast<char*>(p.C) + row * pitch + static_cast<long long>(t.col0) * kElem;
   const bool summed = t.k > 0;
-  // the pieces that this lane stores: piece jj of rows rr + 8 i
-  const int rr = lane >> 2, jj = lane & 3;
-  const uint32_t from = stage + rr * kGroupedChunkBytes + ((jj ^ ((rr >> 1) & 3)) << 4);
-  const uint32_t to = stage + lane * kGroupedChunkBytes;
-  const int swz = (lane >> 1) & 3;
   uint32_t v[kCols];
   auto load = [&](int c) {
     if constexpr (kCols == 32) tmem_ld_32x32b_x32(tbase + c, v);
     else tmem_ld_32x32b_x16(tbase + c, v);
   };
-  if (summed) load(part * kCols);
+  if (summed) load(part * kCols);  // on its way beside the scales
+  long long row;
+  // The scales' product alpha; where it leaves FP32's normal range although neither scale is zero, alpha is the smaller
+  // scale, and the sums are multiplied by the larger one, beta, first.
+  float alpha = 1.f, beta = 1.f;
+  bool twice = false;  // a row of this warp has a beta
+  if constexpr (MODE == GMode::WGRAD) {
+    row = static_cast<long long>(t.g) * p.m + t.row0 + first;
+  } else {
+    row = t.row0 + first;
+    if (t.k > 0) {
+      const float g = p.group_scale ? __ldcg(p.group_scale + t.g) : 1.f;
+      const float r = p.row_scale && lane < nrows ? __ldcg(p.row_scale + row + lane) : 1.f;
+      alpha = g * r;
+      if (g != 0.f && r != 0.f && (fabsf(alpha) < 0x1p-126f || fabsf(alpha) == INFINITY)) {
+        const bool larger = fabsf(g) > fabsf(r);
+        alpha = larger ? r : g;
+        beta = larger ? g : r;
+      }
+      twice = __any_sync(0xffffffffu, beta != 1.f);
+    }
+  }
+  const long long pitch = p.ldc * kElem;
+  char* out = static_cast<char*>(p.C) + row * pitch + static_cast<long long>(t.col0) * kElem;
+  // the pieces that this lane stores: piece jj of rows rr + 8 i
+  const int rr = lane >> 2, jj = lane & 3;
+  const uint32_t from = stage + rr * kGroupedChunkBytes + ((jj ^ ((rr >> 1) & 3)) << 4);
+  const uint32_t to = stage + lane * kGroupedChunkBytes;
+  const int swz = (lane >> 1) & 3;
 #pragma unroll 1
   for (int c = part * kCols; c < width; c += 2 * kCols) {
     uint32_t w[16];
     if (summed) tmem_ld_wait();
+    if (MODE != GMode::WGRAD && twice) {
+#pragma unroll
+      for (int j = 0; j < kCols; ++j) v[j] = __float_as_uint(__uint_as_float(v[j]) * beta);
+    }
 #pragma unroll
     for (int j = 0; j < 16; ++j) {
       if constexpr (OUT == Out::F32) {
