@@ -208,6 +208,7 @@ int bw_gemm_grouped(int dtype, const void* A, long long lda, const void* B, int 
   if (rows > 1 && ldc < N) return set_error(BW_ERR_INVALID, "%s: C's row pitch %lld is below N = %d", name, ldc, N);
   if (((reinterpret_cast<uintptr_t>(row_scale) | reinterpret_cast<uintptr_t>(group_scale)) & 3u))
     return set_error(BW_ERR_INVALID, "%s: scales are not aligned to a float", name);
+  if (C == A || C == B) return set_error(BW_ERR_INVALID, "%s: C over an operand", name);
   if (rows == 1) { lda = (K + 15LL) / 16 * 16; ldc = ldc < N ? N : ldc; }  // a single row has no pitch
   if (K > 0) {
     if ((r = check_operand(name, "A", A, lda, rows, K, es)) != BW_OK) return r;
@@ -236,6 +237,7 @@ int bw_gemm_grouped_wgrad(int dtype, const void* X, long long ldx, const void* Y
   if (M == 0 || N == 0) return BW_OK;
   const int oe = out_dtype == BW_OUT_F32 ? 4 : 2;
   if (!D || reinterpret_cast<uintptr_t>(D) % oe) return set_error(BW_ERR_INVALID, "%s: D is null or not aligned to its element", name);
+  if (D == X || D == Y) return set_error(BW_ERR_INVALID, "%s: D over an operand", name);
   if (rows == 1) { ldx = (M + 7LL) / 8 * 8; ldy = (N + 7LL) / 8 * 8; }
   if (rows > 0 && ((r = check_operand(name, "X", X, ldx, rows, M, 2)) != BW_OK ||
                    (r = check_operand(name, "Y", Y, ldy, rows, N, 2)) != BW_OK))

@@ -217,7 +217,7 @@ int bw_gemm_grouped(int dtype, const void* A, long long lda, const void* B, int 
 /* Weight gradient of the above: D[g] = X[rows of g]^T Y[rows of g], zeros for a group without rows.
  * X: rows x M (pitch ldx), Y: rows x N (pitch ldy), dtype BW_DTYPE_F16 or BF16; D: groups x M x N in out_dtype.
  * With X = A, Y = dC it is the gradient of a groups x K x N matrix, with X = dC, Y = A of its
- * transposed form. Alignment: X, Y and their pitches 16 bytes, D its element. */
+ * transposed form. D may not overlap X or Y. Alignment: X, Y and their pitches 16 bytes, D its element. */
 int bw_gemm_grouped_wgrad(int dtype, const void* X, long long ldx, const void* Y, long long ldy, const int* offsets,
                           int groups, void* D, int out_dtype, int rows, int M, int N, void* stream);
 
