@@ -321,12 +321,12 @@ __device__ __forceinline__ Words<VE> encode_e4m3(const float (&y)[VE], float mul
   return q;
 }
 
-// h + r, rounded once. Through FP32 the 16-bit result is the same (where the FP32 sum rounds, the smaller
-// term is too small to matter to the 16-bit one either), takes 7 instructions for 2 elements instead of 1, and is
-// what PACKED = false asks for.
-template <typename T, int VE, bool PACKED = true>
+// h + r, rounded once; 16-bit elements two an instruction. (Through FP32 the result is the same, 7 instructions for 2
+// elements: in the register kernel 4% less to 3% more time over 32 widths and sizes, without a pattern. 16384 x 8192 BF16 to
+// E4M3 140 us so and 145 packed as a captured graph, 146.5 and 143 called one by one; 26214 x 5120 144 / 141.)
+template <typename T, int VE>
 __device__ __forceinline__ void add_residual(Vec<T, VE>& h, const Vec<T, VE>& r) {
-  if constexpr (!PACKED || std::is_same_v<T, float>) {
+  if constexpr (std::is_same_v<T, float>) {
     float f[VE];
 #pragma unroll
     for (int j = 0; j < VE; ++j) f[j] = elem<T>(h, j) + elem<T>(r, j);
@@ -423,9 +423,6 @@ constexpr int kThreadBytes = NV * (sizeof(T) * VE < 4 ? 4 : sizeof(T) * VE);
 template <typename T, typename WT, bool Q8, int VE, int NV, bool SHIFT>
 __global__ void __launch_bounds__(512) k_rmsnorm(const NormParams p, int tpr) {
   constexpr bool kKeep = kThreadBytes<T, VE, NV> <= 64;
-  // 16384 x 8192 BF16 140 us unpacked and 149 packed (the memory serves slower readers better), 4096 x 4096 20.3 / 19.5;
-  // in every other case packed is 2-12% faster
-  constexpr bool kPacked = SHIFT || NV != 4;
   grid_dependency_wait();
   __shared__ SumMax sm[2][32];
   const int per_block = blockDim.x / tpr;
@@ -460,7 +457,7 @@ __global__ void __launch_bounds__(512) k_rmsnorm(const NormParams p, int tpr) {
       if constexpr (!kKeep) fetch(row);
       if (r) {
 #pragma unroll
-        for (int i = 0; i < NV; ++i) add_residual<T, VE, kPacked>(h.v[i], res.v[i]);
+        for (int i = 0; i < NV; ++i) add_residual<T, VE>(h.v[i], res.v[i]);
         if constexpr (SHIFT) h.one = add_as(T{}, h.one, res.one);
       }
       if (p.h) store_row(static_cast<T*>(p.h) + row * p.ldh, c, h);
@@ -538,8 +535,10 @@ __device__ __forceinline__ void load_staged(const uint8_t* row, const Columns<VE
 
 // k_rmsnorm for rows over 128 vectors which leave lanes idle there, which start behind a boundary, or which are
 // too long for its registers: a block takes one row at a time out of its ring. Both measured, us, in registers / staged
-// (BF16 to E4M3 with residual): 23763 x 1088 39 / 36, 19407 x 2498 75 / 59, 10000 x 5000 67 / 56, 3564 x 9553 78 / 40; rows that
-// fill the lanes: 16384 x 8192 140 / 163, 32768 x 4000 140 / 160.
+// (BF16 to E4M3 with residual): behind a boundary 19407 x 2498 75 / 59, 3564 x 9553 78 / 40; whole vectors 15252 x 8800 186 / 165 (one
+// block an SM), 16384 x 8192 147 / 164, 26214 x 5120 142 / 160. Where the line lies for whole vectors (1700 of an SM's 2048 in use, below):
+// time in registers over time staged, 12 to 128 million elements at 33 widths from 1088 to 16384, both outputs. With a
+// residual 0.86-1.03 (mean 0.96) above the line and 0.83-1.22 (0.99) under it; without one 0.93-1.27 (1.07) and 0.86-1.61 (1.12).
 template <typename T, typename WT, bool Q8, int VE, int NV, bool SHIFT>
 __global__ void __launch_bounds__(512) k_rmsnorm_staged(const NormParams p) {
   constexpr bool kKeep = kThreadBytes<T, VE, NV> <= 64;
