@@ -1030,8 +1030,8 @@ struct Shape {
 // 2.6 / 2.8, 300 x 2048 3.2 / 3.2, 150 x 8192 4.6 / 3.8, 1200 x 8192 16.2 / 12.9); fewer also where a warp's
 // granularity would leave over an eighth more of them idle.
 constexpr int kMaxThreads = 512;
-Shape row_shape(long long rows, long long nvec, int want, int max_nv, int min_tpr) {
-  if (rows * nvec <= 148LL * 512) want = 1;
+Shape row_shape(long long rows, long long nvec, int want, int max_nv, int min_tpr, int sms) {
+  if (rows * nvec <= sms * 512LL) want = 1;
   int nv = want;
   while (nv <= max_nv && nvec > static_cast<long long>(nv) * kMaxThreads) nv *= 2;
   if (nv > max_nv) return {0, 0, 0, 0};
@@ -1148,17 +1148,17 @@ int launch_norm(const NormParams& p, cudaStream_t s, const DeviceState& d) {
   constexpr int kMaxNv = VE == 1 ? 16 : sizeof(T) == 4 ? 8 : 4;
   const long long nvec = SHIFT ? p.cols / VE : (p.cols + VE - 1LL) / VE;
   if constexpr (VE > 1) {
-    const Shape sh = row_shape(p.rows, nvec, 4, kMaxNv, 1);
+    const Shape sh = row_shape(p.rows, nvec, 4, kMaxNv, 1, d.sms);
     // rows of whole vectors whose blocks leave few of an SM's 512 x 4 vectors unused
     const bool full = !SHIFT && sh.nv == 4 && kMaxThreads / sh.block * nvec >= 1700;
-    if (nvec > 128 && p.rows * nvec > 148LL * 512 && !full) {
+    if (nvec > 128 && p.rows * nvec > d.sms * 512LL && !full) {
       const Staging g = row_staging(nvec, 4, sizeof(T) == 4 ? 8 : 4, p.res ? 2 : 1, 768);
       if (g.depth > 0 && g.nv == 4) return launch_staged<k_rmsnorm_staged<T, WT, Q8, VE, 4, SHIFT>, SHIFT>(p, g, s, d);
       if constexpr (sizeof(T) == 4)
         if (g.depth > 0) return launch_staged<k_rmsnorm_staged<T, WT, Q8, VE, 8, SHIFT>, SHIFT>(p, g, s, d);
     }
   }
-  const Shape sh = row_shape(p.rows, nvec, SHIFT && nvec <= 32 ? 1 : 4, kMaxNv, SHIFT ? 16 : 1);
+  const Shape sh = row_shape(p.rows, nvec, SHIFT && nvec <= 32 ? 1 : 4, kMaxNv, SHIFT ? 16 : 1, d.sms);
   if (sh.nv == 0) {
     constexpr int WVE = SHIFT ? 1 : VE;
     BW_CUDA(launch_dependent(k_rmsnorm_wide<T, WT, Q8, WVE>, dim3(static_cast<unsigned>(p.rows)), 1024, 0, s, p));
@@ -1278,18 +1278,19 @@ int norm_impl(const void* x, long long ldx, const void* residual, long long ldr,
   return dispatch_weight<__nv_bfloat16>(p, q8, s, *d);
 }
 
-// Slabs of the weight gradient, one a block: a function of the sizes alone, so that the sums (and the
-// workspace) are the same on every device. 512 threads are resident on an SM (of 148) with this
+// Slabs of the weight gradient that the workspace has room for, one a block: a function of the sizes alone, so that the
+// workspace is the same on every device and for every layout. 512 threads are resident on an SM (of 148) with this
 // kernel's registers (640 with the staged one's), and a block has one for 16 columns, or 256 for short rows; more
 // slabs wait for those to end (a whole second wave, 37476 x 3519 BF16: 267 us with 296, 411 with 338) and write more partial
 // sums (16384 x 8192 BF16: 180 us with 148, 199 with 592).
 int grad_slabs(long long rows, long long cols) {
   long long most = 296;
+  constexpr int kSms = 148;
   if (cols > 512 && cols <= 16384) {
     const int threads = cols > 8192 ? 512 : static_cast<int>((cols + 511) / 512 * 32);
-    most = 148 * ((threads > 256 ? 640 : 512) / threads);
+    most = kSms * ((threads > 256 ? 640 : 512) / threads);
   }
-  if (cols <= 16384 && most > rows / 4) most = rows / 4 > 148 ? rows / 4 : 148;
+  if (cols <= 16384 && most > rows / 4) most = rows / 4 > kSms ? rows / 4 : kSms;
   return static_cast<int>(rows < most ? rows : most);
 }
 
@@ -1299,14 +1300,14 @@ int sum_slabs(const NormGradParams& p, float* dw, cudaStream_t s) {
   return BW_OK;
 }
 
-// A slab (block) for every row up to the workspace's slabs, and no more blocks than one wave of 148 SMs
-// holds by its ring and registers.
+// A slab (block) for every row up to the workspace's slabs, and no more blocks than one wave holds by its
+// ring and registers.
 template <auto KERN, bool SHIFT>
-int launch_grad_staged(NormGradParams p, const Staging& g, float* dw, cudaStream_t s) {
+int launch_grad_staged(NormGradParams p, const Staging& g, float* dw, cudaStream_t s, const DeviceState& d) {
   int per_sm = 0;
   const int r = staged_resident<KERN>(g, &per_sm);
   if (r != BW_OK) return r;
-  int most = 148 * per_sm;
+  int most = d.sms * per_sm;
   if (most > p.slabs) most = p.slabs;
   if (SHIFT && most > 8) most = most / 8 * 8;
   p.slabs = p.rows < most ? static_cast<int>(p.rows) : most;
@@ -1316,26 +1317,26 @@ int launch_grad_staged(NormGradParams p, const Staging& g, float* dw, cudaStream
 }
 
 template <typename T, typename WT, int VE, bool SHIFT>
-int launch_grad(NormGradParams p, float* dw, cudaStream_t s) {
+int launch_grad(NormGradParams p, float* dw, cudaStream_t s, const DeviceState& d) {
   constexpr int kMaxNv = VE == 1 ? 16 : sizeof(T) == 4 ? 8 : 4;
   const long long nvec = SHIFT ? p.cols / VE : (p.cols + VE - 1LL) / VE;
   if constexpr (VE > 1) {
     if (nvec > 64 && p.rows >= 8LL * p.slabs) {
       constexpr int kNv = sizeof(T) == 4 ? 4 : 2;
       const Staging g = row_staging(nvec, kNv, 4, p.dres ? 3 : 2, 512);
-      if (g.depth > 0 && g.nv == kNv) return launch_grad_staged<k_rmsnorm_grad_staged<T, WT, VE, kNv, SHIFT>, SHIFT>(p, g, dw, s);
+      if (g.depth > 0 && g.nv == kNv) return launch_grad_staged<k_rmsnorm_grad_staged<T, WT, VE, kNv, SHIFT>, SHIFT>(p, g, dw, s, d);
       if constexpr (kNv == 2)
-        if (g.depth > 0) return launch_grad_staged<k_rmsnorm_grad_staged<T, WT, VE, 4, SHIFT>, SHIFT>(p, g, dw, s);
+        if (g.depth > 0) return launch_grad_staged<k_rmsnorm_grad_staged<T, WT, VE, 4, SHIFT>, SHIFT>(p, g, dw, s, d);
     }
   }
   // 32 bytes of a row a thread (it fetches ahead then), 64 for long sums in FP32
-  const Shape sh = row_shape(p.rows, nvec, sizeof(T) == 4 && p.rows >= 2048 ? 4 : 2, kMaxNv, SHIFT ? 16 : 1);
+  const Shape sh = row_shape(p.rows, nvec, sizeof(T) == 4 && p.rows >= 2048 ? 4 : 2, kMaxNv, SHIFT ? 16 : 1, d.sms);
   if (sh.nv == 0) {
     // the weight gradient first: dx may be written over dy or h
     BW_CUDA(launch_dependent(k_rmsnorm_dw_wide<T>, dim3(static_cast<unsigned>((p.cols + 255LL) / 256), p.slabs), 256, 0, s, p));
     BW_CUDA(launch_dependent(k_rmsnorm_grad_wide<T, WT>, dim3(static_cast<unsigned>(p.rows)), 1024, 0, s, p));
   } else {
-    if (sh.tpr > 32 && p.slabs > 148 * (kMaxThreads / sh.block)) p.slabs = 148 * (kMaxThreads / sh.block);
+    if (sh.tpr > 32 && p.slabs > d.sms * (kMaxThreads / sh.block)) p.slabs = d.sms * (kMaxThreads / sh.block);
     const long long groups = (p.rows + sh.groups - 1) / sh.groups;
     if (groups <= p.slabs) p.slabs = static_cast<int>(groups);  // a row each
     else if (SHIFT && sh.groups < 8) p.slabs = p.slabs / 8 * 8;  // a stride of whole phases
@@ -1357,24 +1358,24 @@ int launch_grad(NormGradParams p, float* dw, cudaStream_t s) {
 }
 
 template <typename T, typename WT>
-int dispatch_grad(NormGradParams p, float* dw, cudaStream_t s) {
+int dispatch_grad(NormGradParams p, float* dw, cudaStream_t s, const DeviceState& d) {
   constexpr int VE = 16 / sizeof(T);
   const int e = sizeof(T);
   const RowsOf t[] = {{p.h, p.ldh, e}, {p.dy, p.lddy, e}, {p.dres, p.lddr, e}, {p.dx, p.lddx, e}};
   switch (row_access(t, VE, p.cols, &p.phase)) {
     case Access::ALIGNED:
-      if (aligned16(p.w)) return launch_grad<T, WT, VE, false>(p, dw, s);
+      if (aligned16(p.w)) return launch_grad<T, WT, VE, false>(p, dw, s, d);
       [[fallthrough]];
-    case Access::SHIFTED: return launch_grad<T, WT, VE, true>(p, dw, s);
-    default: return launch_grad<T, WT, 1, false>(p, dw, s);
+    case Access::SHIFTED: return launch_grad<T, WT, VE, true>(p, dw, s, d);
+    default: return launch_grad<T, WT, 1, false>(p, dw, s, d);
   }
 }
 
 template <typename T>
-int dispatch_grad_weight(const NormGradParams& p, float* dw, cudaStream_t s) {
+int dispatch_grad_weight(const NormGradParams& p, float* dw, cudaStream_t s, const DeviceState& d) {
   if constexpr (sizeof(T) < 4)
-    if (p.w_f32) return dispatch_grad<T, float>(p, dw, s);
-  return dispatch_grad<T, T>(p, dw, s);
+    if (p.w_f32) return dispatch_grad<T, float>(p, dw, s, d);
+  return dispatch_grad<T, T>(p, dw, s, d);
 }
 
 }  // namespace
@@ -1455,9 +1456,9 @@ int bw_rmsnorm_backward(const void* dy, long long lddy, const void* h, long long
   p.slabs = grad_slabs(rows, cols);
   p.status = d->status;
   p.budget_ns = wait_budget_ns();
-  if (dtype == BW_DTYPE_F32) return dispatch_grad_weight<float>(p, dweight, s);
-  if (dtype == BW_DTYPE_F16) return dispatch_grad_weight<__half>(p, dweight, s);
-  return dispatch_grad_weight<__nv_bfloat16>(p, dweight, s);
+  if (dtype == BW_DTYPE_F32) return dispatch_grad_weight<float>(p, dweight, s, *d);
+  if (dtype == BW_DTYPE_F16) return dispatch_grad_weight<__half>(p, dweight, s, *d);
+  return dispatch_grad_weight<__nv_bfloat16>(p, dweight, s, *d);
 }
 
 }  // extern "C"
