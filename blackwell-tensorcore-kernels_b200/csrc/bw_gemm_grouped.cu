@@ -22,6 +22,20 @@ CUtensorMapDataType map_type(int dtype) {
          : dtype == BW_DTYPE_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
 }
 
+// K atoms a stage and stages of the single-CTA kernel. Narrow tiles hold two atoms a stage: the issuing threads take about
+// 450 cycles a stage, and an atom of such a tile less to load and multiply (one group of 300 x 4096 x 4096, W = 96: E4M3
+// 17.5 -> 14.4 us, BF16 29.0 -> 23.2).
+constexpr int atoms_a_stage(int W) { return W <= 128 ? 2 : 1; }
+constexpr int stage_bytes(int W) { return atoms_a_stage(W) * (kBM + W) * kSlabBytes; }
+constexpr int stages_of(int W, int groups) { return (kMaxSmem - grouped_tail_bytes(groups)) / stage_bytes(W); }
+constexpr bool stages_within(int lo, int hi) {
+  for (int W = 64; W <= 256; W += 16)
+    if (stages_of(W, kMaxGroups) < lo || stages_of(W, 1) > hi) return false;
+  return true;
+}
+static_assert(stages_within(3, kGroupedMaxStages) && !stages_within(4, kGroupedMaxStages) && !stages_within(3, kGroupedMaxStages - 1),
+              "3 to kGroupedMaxStages stages");
+
 // Tile rows that the output can have at most, and that it has when the rows spread evenly.
 long long max_tile_rows(int rows, int groups, int tm) {
   return rows / tm + (groups < rows ? groups : rows);
@@ -90,13 +104,9 @@ int launch(const Operands& o, int dtype, GroupedParams p, cudaStream_t s, const 
   p.W = pair ? 256 : tile_width(p, mt, MODE == GMode::ROWS_NK ? 16 : 64, wgrad, d);
   const long long most = (wgrad ? mt : max_tile_rows(p.rows, p.groups, tm)) * ((p.n + p.W - 1) / p.W);
   if (most >= (1LL << 31) - 4096) return set_error(BW_ERR_INVALID, "grouped GEMM: %lld output tiles exceed the index range", most);
-  // narrow tiles hold two K atoms a stage: the issuing threads take about 450 cycles a stage, and an
-  // atom of such a tile less to load and multiply (one group of 300 x 4096 x 4096, W = 96: E4M3 17.5 -> 14.4 us,
-  // BF16 29.0 -> 23.2)
-  p.sub = p.W <= 128 ? 2 : 1;
-  p.stage_bytes = pair ? kPairStageBytes : p.sub * (kBM + p.W) * kSlabBytes;
-  p.stages = pair ? kPairStages : (kMaxSmem - grouped_tail_bytes(p.groups)) / p.stage_bytes;
-  if (p.stages > kGroupedMaxStages) p.stages = kGroupedMaxStages;
+  p.sub = atoms_a_stage(p.W);
+  p.stage_bytes = pair ? kPairStageBytes : stage_bytes(p.W);
+  p.stages = pair ? kPairStages : stages_of(p.W, p.groups);
   const int smem = p.stages * p.stage_bytes + grouped_tail_bytes(p.groups);
   CUtensorMap ta{}, ta16{}, tb{};
   if ((wgrad ? p.rows : p.k) > 0) {

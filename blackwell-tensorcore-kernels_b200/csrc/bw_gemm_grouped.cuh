@@ -27,7 +27,7 @@ constexpr int kGroupedEpiWarps = 8;   // two for each 32 lanes of Tensor Memory
 constexpr int kGroupedThreads = 32 * (2 + kGroupedEpiWarps + 1);  // producer, MMA, epilogue, tail warp
 constexpr int kGroupedChunkBytes = 64;                             // of a row, staged at a time
 constexpr int kGroupedStageBytes = 32 * kGroupedChunkBytes;        // staging of one epilogue warp
-constexpr int kGroupedMaxStages = 10;
+constexpr int kGroupedMaxStages = 6;
 
 struct GroupedParams {
   void* C;                   // WGRAD: D
@@ -344,7 +344,7 @@ __device__ __forceinline__ bool slab_is_cut(int left, int slab) { return left < 
 
 // Groups of few rows: bound by HBM, which every weight leaves once (64 matrices of 4096 x 2048 E4M3, 16 rows each:
 // 85-90 us, 6.0-6.5 TB/s of the measured 6.5). Persistent, one CTA an SM: warp 0 streams k-slabs into
-// a ring of 3 to 10 stages, warp 1 multiplies, warps 2-9 store one tile while the next is summed in the
+// a ring of 3 to 6 stages, warp 1 multiplies, warps 2-9 store one tile while the next is summed in the
 // other half of Tensor Memory. A tile has 128 rows however few count: their products cost nothing while the weights
 // arrive, and narrower tiles would read them again.
 // One CTA a tile of 128 x W (W <= 256; a multiple of 16, for an N-contiguous B of 64).

@@ -209,8 +209,8 @@ int bw_rmsnorm_backward(const void* dy, long long lddy, const void* h, long long
  * graph replays with new sizes). Empty groups are allowed. Rows before offsets[0] and behind
  * offsets[groups] are left as they were. Offsets outside 0..rows count as the nearest of the two, one below its
  * predecessor as its predecessor. 1 <= groups <= 1024. K = 0 writes zeros. C may not overlap A or B.
- * Alignment: A, B 16 bytes, as are lda, and B's rows (K or N elements); C its element (16- or
- * 32-byte aligned rows store faster). */
+ * Alignment: A, B 16 bytes, as are lda, and B's rows (K or N elements); C its element
+ * (16-byte aligned rows store faster). */
 int bw_gemm_grouped(int dtype, const void* A, long long lda, const void* B, int b_transposed, const int* offsets,
                     int groups, const float* row_scale, const float* group_scale, void* C, long long ldc,
                     int out_dtype, int rows, int N, int K, void* stream);
