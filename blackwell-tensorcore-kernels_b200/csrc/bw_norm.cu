@@ -323,7 +323,7 @@ __device__ __forceinline__ Words<VE> encode_e4m3(const float (&y)[VE], float mul
 
 // h + r, rounded once; 16-bit elements two an instruction. (Through FP32 the result is the same, 7 instructions for 2
 // elements: in the register kernel 4% less to 3% more time over 32 widths and sizes, without a pattern. 16384 x 8192 BF16 to
-// E4M3 140 us so and 145 packed as a captured graph, 146.5 and 143 called one by one; 26214 x 5120 144 / 141.)
+// E4M3 140 us so and 145-149 packed as a captured graph, 146.5 and 143 called one by one; 26214 x 5120 144 / 141.)
 template <typename T, int VE>
 __device__ __forceinline__ void add_residual(Vec<T, VE>& h, const Vec<T, VE>& r) {
   if constexpr (std::is_same_v<T, float>) {
