@@ -16,6 +16,8 @@
 // must not meet a zero). The tensor maps of B are 3-D, so a k-slab that reaches over K reads zeros, not
 // the next matrix.
 #pragma once
+#include <type_traits>
+
 #include "bw_gemm_kernel.cuh"
 
 namespace bw {
@@ -232,24 +234,17 @@ __device__ __forceinline__ void grouped_epilogue(const GroupedParams& p, const G
   };
   if (summed) load(part * kCols);  // on its way beside the scales
   long long row;
-  // The scales' product alpha; where it leaves FP32's normal range although neither scale is zero, alpha is the smaller
-  // scale, and the sums are multiplied by the larger one, beta, first.
-  float alpha = 1.f, beta = 1.f;
-  bool twice = false;  // a row of this warp has a beta
+  float alpha = 1.f;
+  bool twice = false;  // the scales' product leaves FP32's normal range in one of this warp's rows
   if constexpr (MODE == GMode::WGRAD) {
     row = static_cast<long long>(t.g) * p.m + t.row0 + first;
   } else {
     row = t.row0 + first;
     if (t.k > 0) {
-      const float g = p.group_scale ? __ldcg(p.group_scale + t.g) : 1.f;
-      const float r = p.row_scale && lane < nrows ? __ldcg(p.row_scale + row + lane) : 1.f;
-      alpha = g * r;
-      if (g != 0.f && r != 0.f && (fabsf(alpha) < 0x1p-126f || fabsf(alpha) == INFINITY)) {
-        const bool larger = fabsf(g) > fabsf(r);
-        alpha = larger ? r : g;
-        beta = larger ? g : r;
-      }
-      twice = __any_sync(0xffffffffu, beta != 1.f);
+      if (p.group_scale) alpha *= __ldcg(p.group_scale + t.g);
+      if (p.row_scale && lane < nrows) alpha *= __ldcg(p.row_scale + row + lane);
+      if (p.group_scale && p.row_scale)  // exponent field 0 or 255
+        twice = __any_sync(0xffffffffu, (__float_as_uint(alpha) << 1) - 0x01000000u >= 0xfe000000u);
     }
   }
   const long long pitch = p.ldc * kElem;
@@ -259,61 +254,76 @@ __device__ __forceinline__ void grouped_epilogue(const GroupedParams& p, const G
   const uint32_t from = stage + rr * kGroupedChunkBytes + ((jj ^ ((rr >> 1) & 3)) << 4);
   const uint32_t to = stage + lane * kGroupedChunkBytes;
   const int swz = (lane >> 1) & 3;
+  float beta = 1.f;
+  auto store = [&](auto scaled_twice) {
 #pragma unroll 1
-  for (int c = part * kCols; c < width; c += 2 * kCols) {
-    uint32_t w[16];
-    if (summed) tmem_ld_wait();
-    if (MODE != GMode::WGRAD && twice) {
+    for (int c = part * kCols; c < width; c += 2 * kCols) {
+      uint32_t w[16];
+      if (summed) tmem_ld_wait();
+      if constexpr (decltype(scaled_twice)::value) {
 #pragma unroll
-      for (int j = 0; j < kCols; ++j) v[j] = __float_as_uint(__uint_as_float(v[j]) * beta);
-    }
-#pragma unroll
-    for (int j = 0; j < 16; ++j) {
-      if constexpr (OUT == Out::F32) {
-        w[j] = __float_as_uint(__uint_as_float(v[j]) * alpha);
-      } else {
-        const __nv_bfloat162 two =
-            __floats2bfloat162_rn(__uint_as_float(v[2 * j]) * alpha, __uint_as_float(v[2 * j + 1]) * alpha);
-        w[j] = *reinterpret_cast<const uint32_t*>(&two);
+        for (int j = 0; j < kCols; ++j) v[j] = __float_as_uint(__uint_as_float(v[j]) * beta);
       }
-      if (!summed) w[j] = 0;
-    }
-    if (summed) {  // the next columns come while these are stored
-      if (c + 2 * kCols < width) load(c + 2 * kCols);
-      else release();
-    }
 #pragma unroll
-    for (int j = 0; j < 4; ++j) st_shared_v4(to + ((j ^ swz) << 4), w[4 * j], w[4 * j + 1], w[4 * j + 2], w[4 * j + 3]);
-    __syncwarp();
-    const int have = width - c - jj * kPiece;  // columns of this lane's pieces that exist
-    char* dst = out + rr * pitch + (c + jj * kPiece) * kElem;
-    if (p.vec == 16 && width - c >= kCols) {
-      uint4 x[4];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) x[i] = ld_shared_v4(from + i * 8 * kGroupedChunkBytes);
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-        if (rr + 8 * i < nrows) st_global_v4(dst + 8 * i * pitch, x[i]);
-    } else {
-#pragma unroll 1
-      for (int i = 0; i < 4; ++i) {
-        if (rr + 8 * i >= nrows || have <= 0) continue;
-        const uint4 x = ld_shared_v4(from + i * 8 * kGroupedChunkBytes);
-        char* at = dst + 8 * i * pitch;
-        if (p.vec == 16 && have >= kPiece) {
-          st_global_v4(at, x);
+      for (int j = 0; j < 16; ++j) {
+        if constexpr (OUT == Out::F32) {
+          w[j] = __float_as_uint(__uint_as_float(v[j]) * alpha);
         } else {
-          const uint32_t e[4] = {x.x, x.y, x.z, x.w};
+          const __nv_bfloat162 two =
+              __floats2bfloat162_rn(__uint_as_float(v[2 * j]) * alpha, __uint_as_float(v[2 * j + 1]) * alpha);
+          w[j] = *reinterpret_cast<const uint32_t*>(&two);
+        }
+        if (!summed) w[j] = 0;
+      }
+      if (summed) {  // the next columns come while these are stored
+        if (c + 2 * kCols < width) load(c + 2 * kCols);
+        else release();
+      }
 #pragma unroll
-          for (int k = 0; k < kPiece; ++k) {
-            if (k >= have) break;
-            if constexpr (OUT == Out::F32) reinterpret_cast<uint32_t*>(at)[k] = e[k];
-            else reinterpret_cast<uint16_t*>(at)[k] = static_cast<uint16_t>(e[k / 2] >> (16 * (k & 1)));
+      for (int j = 0; j < 4; ++j) st_shared_v4(to + ((j ^ swz) << 4), w[4 * j], w[4 * j + 1], w[4 * j + 2], w[4 * j + 3]);
+      __syncwarp();
+      const int have = width - c - jj * kPiece;  // columns of this lane's pieces that exist
+      char* dst = out + rr * pitch + (c + jj * kPiece) * kElem;
+      if (p.vec == 16 && width - c >= kCols) {
+        uint4 x[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x[i] = ld_shared_v4(from + i * 8 * kGroupedChunkBytes);
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (rr + 8 * i < nrows) st_global_v4(dst + 8 * i * pitch, x[i]);
+      } else {
+#pragma unroll 1
+        for (int i = 0; i < 4; ++i) {
+          if (rr + 8 * i >= nrows || have <= 0) continue;
+          const uint4 x = ld_shared_v4(from + i * 8 * kGroupedChunkBytes);
+          char* at = dst + 8 * i * pitch;
+          if (p.vec == 16 && have >= kPiece) {
+            st_global_v4(at, x);
+          } else {
+            const uint32_t e[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+            for (int k = 0; k < kPiece; ++k) {
+              if (k >= have) break;
+              if constexpr (OUT == Out::F32) reinterpret_cast<uint32_t*>(at)[k] = e[k];
+              else reinterpret_cast<uint16_t*>(at)[k] = static_cast<uint16_t>(e[k / 2] >> (16 * (k & 1)));
+            }
           }
         }
       }
+      __syncwarp();
     }
-    __syncwarp();
+  };
+  if (MODE != GMode::WGRAD && twice) {
+    // alpha becomes the smaller scale, and the sums are multiplied by the larger one, beta, first (a loop of its own: 32
+    // products more, or a branch around them, take 4% of a call that is bound by this loop)
+    const float g = __ldcg(p.group_scale + t.g), r = lane < nrows ? __ldcg(p.row_scale + row + lane) : 1.f;
+    if (g != 0.f && r != 0.f) {
+      alpha = fabsf(g) > fabsf(r) ? r : g;
+      beta = fabsf(g) > fabsf(r) ? g : r;
+    }
+    store(std::true_type{});
+  } else {
+    store(std::false_type{});
   }
 }
 
@@ -651,9 +661,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGroupedThreads, 1)
   uint64_t* accempty = accfull + 2;
   uint64_t* teardown = accempty + 2;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(teardown + 1);
-  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
-  volatile int* peer_abort = reinterpret_cast<volatile int*>(tmem_slot + 2);  // the other CTA's abort flag, written at the end
-  uint32_t* loads = tmem_slot + 3;  // what this CTA's producer leaves: slabs issued, bytes of `peer_units`
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 2);
+  volatile int* peer_abort = reinterpret_cast<volatile int*>(tmem_slot + 3);  // the other CTA's abort flag, written at the end
+  uint32_t* loads = tmem_slot + 4;  // what this CTA's producer leaves: slabs issued, bytes of `peer_units`
   int* bounds = reinterpret_cast<int*>(tmem_slot + 8);
   int* tiles = bounds + p.groups + 1;
 
@@ -894,7 +904,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGroupedThreads, 1)
   if (threadIdx.x == 0 && *abort_flag) st_shared_cluster(mapa_shared(smem_u32(const_cast<int*>(peer_abort)), rank ^ 1), 1);
   __syncwarp();
   cluster_sync();
-  if (*abort_flag || *peer_abort) {
+  if (warp == 1) {
+    __syncwarp();
+    tc_fence_after();
+    tmem_dealloc_pair(tmem_base, 512);
+  }
+  if (*reinterpret_cast<volatile unsigned long long*>(tmem_slot + 2) != 0) {  // both flags
     // A wait timed out in one of the CTAs: both come here. The loads of both land before either ends. They are counted on
     // the leader's full[s], which expects a slab's bytes from both CTAs as soon as the leader issues its half; where only one
     // has issued the stage's last slab, the phase is made to expect that one's bytes alone. (The two are
@@ -913,11 +928,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kGroupedThreads, 1)
     }
     __syncthreads();
     cluster_sync();
-  }
-  if (warp == 1) {
-    __syncwarp();
-    tc_fence_after();
-    tmem_dealloc_pair(tmem_base, 512);
   }
 }
 
