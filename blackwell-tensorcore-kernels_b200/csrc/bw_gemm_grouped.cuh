@@ -599,7 +599,7 @@ __global__ void __launch_bounds__(kGroupedThreads, 1)
 
 // ------------------------------------------------------------------------------------
 // CTA pairs: 256 x 256 tiles for groups with many rows, bound by the tensor cores (91-92% of the active cycles; 8 x
-// 4096 rows of 4096 x 2048 BF16 347 us = 1585 TFLOP/s at 1.50 GHz, E4M3 8 x 2048 of 8192 x 4096 365 us = 3012): a pair
+// 4096 rows of 4096 x 2048 BF16 348 us = 1581 TFLOP/s at 1.47 GHz, E4M3 8 x 2048 of 8192 x 4096 371 us = 2967 at 1.43): a pair
 // moves a third less per product than two single CTAs, which L2 cannot feed at that rate. As in bw_gemm_pair.cuh, each CTA of a pair
 // loads its 128 rows of A and 128 columns of B, the leader's MMA thread multiplies both halves, and a
 // pipeline stage holds two swizzle atoms of K. Barriers: full[s], fixed[s] and accempty[b] count in

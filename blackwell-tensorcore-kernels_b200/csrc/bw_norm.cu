@@ -12,9 +12,9 @@
 // in registers (packed in its own type: h is rounded to it anyway, and h w in FP32) between its
 // reduction and its output. max |y| needs no second reduction: y_j = (h_j w_j) rstd and rounding is
 // monotonic, so max |y| = max |h w| * rstd exactly, and both sums travel through one reduction.
-// Statistics and sums are FP32. Measured, 16384 x 8192 BF16 with residual: to E4M3 140 us (6.7 TB/s of
-// the 7 bytes an element), gradient 155 us (6.9 TB/s of 8 bytes); 131072 x 128 BF16 to BF16 10.5 us
-// (6.4 TB/s); 16384 x 8191 to E4M3, rows at every alignment, 144 us; one row of 8192 2.8 us.
+// Statistics and sums are FP32. Measured, 16384 x 8192 BF16 with residual: to E4M3 137 us alone (6.9 TB/s of
+// the 7 bytes an element), 143 called one by one, 150 back to back in a graph; gradient 155 us (6.9 TB/s of 8 bytes); 131072 x
+// 128 BF16 to BF16 10.4 us (6.5 TB/s); 16384 x 8191 to E4M3, rows at every alignment, 144 us; one row of 8192 2.6 us.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_fp8.h>
@@ -1069,8 +1069,8 @@ Access row_access(const RowsOf (&t)[N], int ve, long long cols, int* phase) {
   return aligned ? Access::ALIGNED : same ? Access::SHIFTED : Access::SCALAR;
 }
 
-// As many blocks as are resident at once (16384 x 8192 BF16: 141 us; with one more a SM 143 us, and with
-// a few left over twice as long), each with its share of the rows.
+// As many blocks as are resident at once (16384 x 8192 BF16: one more a SM takes 1% longer, a few left over twice as long),
+// each with its share of the rows.
 template <auto KERN, bool SHIFT>
 int launch_rows(const NormParams& p, const Shape& sh, cudaStream_t s, const DeviceState& d) {
   static std::atomic<int> resident[kMaxThreads / 32 + 1] = {};  // by block size, of this kernel; 0: not asked yet

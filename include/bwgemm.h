@@ -170,13 +170,15 @@ size_t bw_sf_offset(int row, int kblock, int K);
  * bw_rmsnorm writes y in x's type; bw_rmsnorm_fp8 writes E4M3 codes and one scale a row, as
  * bw_gemm_grouped takes them: row_scale = amax(|y|) / 448 (1 when the maximum is 0, not finite, or so
  * small that 448 / amax overflows), q = cvt(y * (448 / amax)), satfinite.
+ * (A NaN among a row's y alone, from a weight, keeps its own code and does not count in the maximum.)
  * dtype: BW_DTYPE_F32, F16 or BF16 (x, residual, y, h); weight_dtype: the same or BW_DTYPE_F32.
  * h and rstd may be NULL (not wanted). ld*: row pitches in elements, at least cols. Any alignment
  * to whole elements; 16-byte aligned rows run faster. y and h may each be x's or the residual's own
  * buffer (same type, same pitch), not both the same one; other overlap is not allowed. With y over x and no
- * residual, the h that the gradient needs is gone unless it is asked for. Sums are FP32: a row whose squares
- * sum to more than FP32 holds gets rstd = 0, one with a NaN, or of zeros with eps = 0, gets NaN (codes
- * 0x7f, scale 1). */
+ * residual, the h that the gradient needs is gone unless it is asked for. Sums and h * weight, which is
+ * taken before rstd, are FP32: a row whose squares sum to more than FP32 holds gets rstd = 0, one with a NaN, or of zeros
+ * with eps = 0, gets NaN (codes 0x7f, scale 1); with eps = 0 rows under about 1e-18 lose precision (their squares leave
+ * FP32's normal range). */
 int bw_rmsnorm(const void* x, long long ldx, const void* residual, long long ldr, const void* weight, int dtype,
                int weight_dtype, float eps, void* y, long long ldy, void* h, long long ldh, float* rstd, int rows,
                int cols, void* stream);
@@ -189,7 +191,9 @@ int bw_rmsnorm_fp8(const void* x, long long ldx, const void* residual, long long
  * dresidual (NULL: none) is the gradient that reached h past the norm. dx may be dy's, h's or
  * dresidual's own buffer (same pitch). workspace: device memory of at least
  * bw_rmsnorm_backward_workspace(rows, cols) bytes, the caller's own for as long as the call runs on
- * the stream (calls that may overlap need one each). Rows are summed in an order fixed by the sizes. */
+ * the stream (calls that may overlap need one each). Its size depends on the sizes alone. The order in which rows are summed
+ * depends on sizes, types, alignment, pitches, whether dresidual is given, and the device: the same call gives the same
+ * bits, and a call with other pointers does where these agree. */
 size_t bw_rmsnorm_backward_workspace(int rows, int cols);
 int bw_rmsnorm_backward(const void* dy, long long lddy, const void* h, long long ldh, const void* weight, int dtype,
                         int weight_dtype, const float* rstd, const void* dresidual, long long lddr, void* dx,
