@@ -432,7 +432,7 @@ def rmsnorm(x, weight, residual=None, eps: float = 1e-6, y=None, h=None, rstd=No
         _check(lib().bw_rmsnorm(x.data_ptr(), ldx, _ptr(residual), ldr, weight.data_ptr(), code, wcode, eps,
                                 y.data_ptr(), ldy, _ptr(hout), ldh, rstd.data_ptr(), shape[0], shape[1],
                                 _current_stream(dev)))
-    if h is x and hout is None and y.data_ptr() == x.data_ptr():
+    if h is x and hout is None and y.data_ptr() == x.data_ptr() and shape[0] > 0:  # (of no rows all pointers are null)
         h = None
     return y, h, rstd
 

@@ -99,3 +99,14 @@ def test_gradient_behind_a_norm_in_place(cuda_dev, cols):
     with pytest.raises(bwgemm.BwError, match="different size"):
         bwgemm.rmsnorm_fp8(x, w, q=x.view(torch.uint8)[:, :cols])
     assert torch.equal(x, x0)
+
+
+@pytest.mark.gpu
+def test_no_rows_keep_their_h(cuda_dev):
+    import torch
+
+    x, w = torch.empty(0, 16, device=cuda_dev), torch.ones(16, device=cuda_dev)
+    for kw in ({}, {"y": x}):
+        y, h, rstd = bwgemm.rmsnorm(x, w, **kw)
+        dx, dw = bwgemm.rmsnorm_backward(y, h, w, rstd)
+        assert dx.shape == (0, 16) and bool((dw == 0).all())
